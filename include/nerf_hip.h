@@ -48,8 +48,9 @@ extern "C" {
 /* Version of this interface (2: the training entry points take a `precision` argument; 3: adds
  * nerf_mlp_backward_static; 4: adds nerf_mlp_forward_objects; 5: adds nerf_make_rays_views; 6: the inference entry
  * points accept NERF_PREC_BF16X3 / NERF_PREC_BF16X2; adds nerf_render_rays; nerf_raw2outputs_backward takes g_weights;
- * 7: the training entry points accept NERF_PREC_BF16X3). */
-#define NERF_HIP_ABI_VERSION 7
+ * 7: the training entry points accept NERF_PREC_BF16X3; 8: adds the layer operators nerf_linear, nerf_linear_backward,
+ * nerf_linear_q8, nerf_add_rms_norm, nerf_add_rms_norm_backward and their workspace sizes). */
+#define NERF_HIP_ABI_VERSION 8
 int nerf_hip_abi_version(void);
 const char* nerf_last_error(void);
 
@@ -283,6 +284,64 @@ int nerf_adam_step(int n_tensors, float* const* params_host, const float* const*
                    float* const* exp_avg_host, float* const* exp_avg_sq_host,
                    const long long* numel_host, long long step, float lr, float beta1, float beta2,
                    float eps, float weight_decay, void* stream);
+
+/* ---- layer operators ----------------------------------------------------------------------
+ * The layers of networks that the fused kernels above do not cover (other depths and widths, residual trunks:
+ * NeRF(D, W, ...) of run_nerf_helpers.py:67-119 evaluated layer by layer), each with what surrounds it in one launch.
+ * Sizes, row strides and alignments are free: a matrix is given by its first element and the number of elements from
+ * one row to the next (ld, at least its row's length; columns are contiguous).  Buffers of one call must not overlap,
+ * except that y may be the residual itself.  All sums are float32; results are the same for every call with the same
+ * arguments (no atomics).                                                                                          */
+#define NERF_DT_F32 0
+#define NERF_DT_BF16 1
+#define NERF_DT_F16 2
+
+#define NERF_ACT_NONE 0
+#define NERF_ACT_RELU 1
+#define NERF_ACT_GELU 2       /* z times the integral of the normal distribution up to z (no tanh approximation)     */
+#define NERF_ACT_SILU 3       /* z / (1 + exp(-z))                                                                   */
+
+/* y[M,N] = act(x w^T + bias) + residual, all of type dtype.  x is x0 [M,k0] or, with k1 > 0, the two pieces
+ * [x0 | x1 [M,k1]] side by side (the concatenation behind a skip connection, never formed); w [N, k0+k1] as nn.Linear
+ * holds it; bias [N] or NULL; residual [M,N] or NULL.  z [M,N] or NULL receives the argument of act, which the
+ * backward needs (for relu without a residual y itself serves).  M < 2^31, N and k up to 2^24.                       */
+int nerf_linear(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
+                const void* w, long long ldw, const void* bias, int activation, const void* residual, long long ldr,
+                void* y, long long ldy, void* z, long long ldz, long long M, int N, void* stream);
+
+/* Gradients of nerf_linear for g [M,N] = dL/dy (the residual's gradient is g itself).  z as the forward wrote it (not
+ * read for NERF_ACT_NONE).  dx0 [M,k0], dx1 [M,k1], dw [N,k0+k1] contiguous and db [N] are overwritten; each may be
+ * NULL and is then not computed (x0, x1 are read for dw only, w for dx0 and dx1 only).  With M = 0 dw and db are
+ * zeros.  workspace: nerf_linear_backward_workspace_bytes(...) bytes on a 256-byte boundary, not shared with a call
+ * that may run at the same time.                                                                                     */
+size_t nerf_linear_backward_workspace_bytes(int dtype, long long M, int N, int k0, int k1, int activation);
+int nerf_linear_backward(int dtype, const void* g, long long ldg, const void* z, long long ldz, int activation,
+                         const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
+                         const void* w, long long ldw, void* dx0, long long lddx0, void* dx1, long long lddx1,
+                         void* dw, void* db, long long M, int N, void* workspace, size_t workspace_bytes, void* stream);
+
+/* nerf_linear on 8-bit operands (e4m3: four exponent bits, no infinities, largest 448): xq [M,K] and wq [N,K] hold
+ * numbers that stand for x_scale[m] xq and w_scale[n] wq.  y, bias and residual are of type out_dtype.               */
+int nerf_linear_q8(const void* xq, long long ldx, const float* x_scale, const void* wq, long long ldw,
+                   const float* w_scale, int out_dtype, const void* bias, int activation, const void* residual,
+                   long long ldr, void* y, long long ldy, long long M, int N, int K, void* stream);
+
+/* h = x + residual (residual NULL: h = x), y = w h / sqrt(mean(h^2) + eps) over the N columns of each row.  The sum and
+ * the norm are taken in float32 before h is rounded to dtype.  Exactly one of y [M,N] and q is given: q [M,N] holds y in
+ * e4m3 with scale[M] = max(max|y| / 448, 2^-126), and a row that is not finite reads back as NaN.  h [M,N] and rstd [M]
+ * (1 / sqrt(...), which the backward needs) may be NULL.  N <= 32768.                                                */
+int nerf_add_rms_norm(int dtype, const void* x, long long ldx, const void* residual, long long ldr, const void* w,
+                      float eps, void* h, long long ldh, void* y, long long ldy, void* q, long long ldq,
+                      float* scale, float* rstd, long long M, int N, void* stream);
+
+/* Gradients of nerf_add_rms_norm for gy = dL/dy and gh = dL/dh (what reaches h by the residual stream; NULL = zero):
+ * dx [M,N] is the gradient of x and of the residual, dw [N] the weights'.  Either may be NULL.  h and rstd are the
+ * forward's.  workspace as for nerf_linear_backward (needed for dw).                                                 */
+size_t nerf_add_rms_norm_backward_workspace_bytes(long long M, int N);
+int nerf_add_rms_norm_backward(int dtype, const void* gy, long long ldgy, const void* gh, long long ldgh,
+                               const void* h, long long ldh, const void* w, const float* rstd, void* dx,
+                               long long lddx, void* dw, long long M, int N, void* workspace,
+                               size_t workspace_bytes, void* stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,533 @@
+// Linear layers of any size: C[p, q] = sum_r A(p, r) B(q, r) on the matrix cores with the layer's epilogue, for the
+// three products of a layer y = act(x W^T + b) + r:
+//
+//     forward   C = y   p = sample  q = output   r = input    A = x  [p][r]     B = W [q][r]
+//     dx        C = dx  p = sample  q = input    r = output   A = gz [p][r]     B = W [r][q]   (B reduction-major)
+//     dW        C = dW  p = output  q = input    r = sample   A = gz [r][p]     B = x [r][q]   (both reduction-major)
+//
+// Each operand is read as it lies in memory; the transposition of a reduction-major one happens between LDS and the
+// registers (ds_read_b64_tr_b16 for 16-bit types, single-word reads for float32).  Sums are float32 throughout.
+#pragma once
+#include "common.h"
+
+namespace nerf {
+namespace lin {
+
+enum { F32 = NERF_DT_F32, BF16 = NERF_DT_BF16, F16 = NERF_DT_F16, F8 = 3 };
+constexpr int elem_size(int dt) { return dt == F32 ? 4 : dt == F8 ? 1 : 2; }
+
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x4 __attribute__((ext_vector_type(4)));
+typedef int i32x8 __attribute__((ext_vector_type(8)));
+typedef short s16x4 __attribute__((ext_vector_type(4)));
+typedef short s16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef __bf16 bf16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef __attribute__((address_space(3))) unsigned char lds_u8;
+
+// One piece of the reduction: the input of a layer may come in two pieces side by side.
+struct Seg {
+    const void *a, *b;
+    long long lda, ldb;          // elements between rows of the operand as it lies in memory
+    long long red;               // length of the reduction over this piece
+};
+
+struct GemmArgs {
+    Seg seg[2];
+    int nseg;
+    long long P, Q;              // rows and columns of C
+    int splits;                  // the reduction is cut into this many parts (nseg = 1) ...
+    long long red_part;          // ... of this many elements each (a multiple of the tile's)
+    float* partial;              // [splits][P][Q] float32 sums instead of the epilogue, or null
+    // epilogue: y = act(C s_p s_q + bias) + res; z = the argument of act
+    const void *bias, *res;
+    void *y, *z;
+    long long ldr, ldy, ldz;
+    const float *sp, *sq;        // 8-bit operands: scales of the rows of A and of B
+    int act;
+    int out_dt;                  // type of y, bias, res, z
+    unsigned tiles_p, tiles_q;
+};
+
+// what the three products need of the operands' layouts
+enum Layout { FWD = 0, DX = 1, DW = 2 };
+
+int gemm_f32(int layout, GemmArgs& g, hipStream_t s);
+int gemm_bf16(int layout, GemmArgs& g, hipStream_t s);
+int gemm_f16(int layout, GemmArgs& g, hipStream_t s);
+int gemm_f8(GemmArgs& g, hipStream_t s);
+
+// ---------------------------------------------------------------------------------------------- scalars and epilogue
+__device__ __forceinline__ float ld_elem(const void* p, long long i, int dt) {
+    if (dt == F32) return reinterpret_cast<const float*>(p)[i];
+    if (dt == BF16) return (float)reinterpret_cast<const __bf16*>(p)[i];
+    return (float)reinterpret_cast<const _Float16*>(p)[i];
+}
+__device__ __forceinline__ void st_elem(void* p, long long i, float v, int dt) {
+    if (dt == F32) reinterpret_cast<float*>(p)[i] = v;
+    else if (dt == BF16) reinterpret_cast<__bf16*>(p)[i] = (__bf16)v;
+    else reinterpret_cast<_Float16*>(p)[i] = (_Float16)v;
+}
+// Eight consecutive elements at any element: 16-byte accesses need no alignment on this hardware's global memory.
+template <int DT>
+__device__ __forceinline__ void ld8(const void* p, long long i, float (&v)[8]) {
+    if constexpr (DT == F32) {
+        __builtin_memcpy(v, reinterpret_cast<const float*>(p) + i, 32);
+    } else if constexpr (DT == BF16) {
+        bf16x8 a;
+        __builtin_memcpy(&a, reinterpret_cast<const __bf16*>(p) + i, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
+    } else {
+        f16x8 a;
+        __builtin_memcpy(&a, reinterpret_cast<const _Float16*>(p) + i, 16);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = (float)a[j];
+    }
+}
+template <int DT>
+__device__ __forceinline__ void st8(void* p, long long i, const float (&v)[8]) {
+    if constexpr (DT == F32) {
+        __builtin_memcpy(reinterpret_cast<float*>(p) + i, v, 32);
+    } else if constexpr (DT == BF16) {
+        bf16x8 a;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = (__bf16)v[j];
+        __builtin_memcpy(reinterpret_cast<__bf16*>(p) + i, &a, 16);
+    } else {
+        f16x8 a;
+#pragma unroll
+        for (int j = 0; j < 8; ++j) a[j] = (_Float16)v[j];
+        __builtin_memcpy(reinterpret_cast<_Float16*>(p) + i, &a, 16);
+    }
+}
+
+// The normal distribution's integral, Phi(z) = erfc(-z / sqrt 2) / 2, and exp(-z^2 / 2) beside it.  The tail
+// erfc(x) exp(x^2) is t P(t) with t = 1 / (1 + 0.4 x): P of degree 8, fitted over the whole half line to a relative
+// 1.3e-7 (weighted least squares, reweighted towards equal error).  In float32 z Phi(z) is off by at most 4e-7, and the
+// lower tail keeps its leading digits (2.5e-6 down to z = -5).  About 20 instructions, where erfcf() takes 60.
+__device__ __forceinline__ float exp2_fast(float x) { return __builtin_amdgcn_exp2f(x); }     // 1 ulp; tiny results become 0
+__device__ __forceinline__ float normal_cdf(float z, float& e) {
+    const float x = fabsf(z) * 0.70710678118654752f;
+    const float t = __builtin_amdgcn_rcpf(fmaf(0.4f, x, 1.f));
+    float p = 0.050261341f;
+    p = fmaf(p, t, -0.18289855f);
+    p = fmaf(p, t, 0.16908108f);
+    p = fmaf(p, t, -0.0056041828f);
+    p = fmaf(p, t, 0.14143002f);
+    p = fmaf(p, t, 0.1685423f);
+    p = fmaf(p, t, 0.20784266f);
+    p = fmaf(p, t, 0.22566959f);
+    p = fmaf(p, t, 0.22567587f);
+    e = exp2_fast(x * x * -1.4426950408889634f);
+    const float tail = 0.5f * t * p * e;
+    return z < 0.f ? tail : 1.f - tail;
+}
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp2_fast(z * -1.4426950408889634f)); }
+
+// relu keeps NaN: a comparison that is false for it selects z.
+__device__ __forceinline__ float act_fn(float z, int act) {
+    float e;
+    switch (act) {
+        case NERF_ACT_RELU: return z <= 0.f ? 0.f : z;
+        case NERF_ACT_GELU: return z * normal_cdf(z, e);
+        case NERF_ACT_SILU: return z * sigmoid(z);
+        default: return z;
+    }
+}
+// Beyond +-100 the derivatives are 0 and 1 to the last bit; held there so that an infinite z (float16 reaches it) does
+// not multiply a vanished factor.
+__device__ __forceinline__ float act_grad(float z, int act) {
+    z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
+    switch (act) {
+        case NERF_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
+        case NERF_ACT_GELU: {
+            float e;
+            const float c = normal_cdf(z, e);
+            return fmaf(z * 0.39894228040143268f, e, c);
+        }
+        case NERF_ACT_SILU: {
+            const float p = sigmoid(z);
+            return p * fmaf(z, 1.f - p, 1.f);
+        }
+        default: return 1.f;
+    }
+}
+// the epilogue's types: of the operands, or, for 8-bit operands, named by the call
+template <int DT>
+__device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8], int dt) {
+    if constexpr (DT != F8) ld8<DT>(p, i, v);
+    else if (dt == F32) ld8<F32>(p, i, v);
+    else if (dt == BF16) ld8<BF16>(p, i, v);
+    else ld8<F16>(p, i, v);
+}
+template <int DT>
+__device__ __forceinline__ void store8(void* p, long long i, const float (&v)[8], int dt) {
+    if constexpr (DT != F8) st8<DT>(p, i, v);
+    else if (dt == F32) st8<F32>(p, i, v);
+    else if (dt == BF16) st8<BF16>(p, i, v);
+    else st8<F16>(p, i, v);
+}
+
+// Eight columns of one row.  Both ways out (a whole group by 16-byte accesses, the last columns one by one) share the
+// arithmetic in between.
+template <int DT>
+__device__ __forceinline__ void some8(const void* p, long long i, bool whole, int n, float (&v)[8], int dt) {
+    if (whole) load8<DT>(p, i, v, dt);
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? ld_elem(p, i + j, DT == F8 ? dt : DT) : 0.f;
+    }
+}
+template <int DT>
+__device__ __forceinline__ void put_some8(void* p, long long i, bool whole, int n, const float (&v)[8], int dt) {
+    if (whole) store8<DT>(p, i, v, dt);
+    else {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) if (j < n) st_elem(p, i + j, v[j], DT == F8 ? dt : DT);
+    }
+}
+template <int DT>
+__device__ __forceinline__ void epilogue8(const GemmArgs& g, long long p, long long q, float (&v)[8]) {
+    const bool whole = q + 8 <= g.Q;
+    const int n = whole ? 8 : (int)(g.Q - q);
+    float t[8];
+    if constexpr (DT == F8) {
+        const float s = g.sp[p];
+        some8<F32>(g.sq, q, whole, n, t, F32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = v[j] * s * t[j];
+    }
+    if (g.bias) {
+        some8<DT>(g.bias, q, whole, n, t, g.out_dt);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    if (g.z) put_some8<DT>(g.z, p * g.ldz + q, whole, n, v, g.out_dt);
+    if (g.act == NERF_ACT_RELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_fn(v[j], NERF_ACT_RELU);
+    } else if (g.act == NERF_ACT_GELU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_fn(v[j], NERF_ACT_GELU);
+    } else if (g.act == NERF_ACT_SILU) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] = act_fn(v[j], NERF_ACT_SILU);
+    }
+    if (g.res) {
+        some8<DT>(g.res, p * g.ldr + q, whole, n, t, g.out_dt);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += t[j];
+    }
+    put_some8<DT>(g.y, p * g.ldy + q, whole, n, v, g.out_dt);
+}
+
+// ---------------------------------------------------------------------------------------------- one operand's tile
+// A tile holds 128 bytes of reduction (BK elements) for OUT rows of C (columns for B).  In LDS it lies as in memory,
+// [OUT][BK] or, reduction-major, [BK][OUT], in 16-byte chunks.  The chunks of a row are permuted so that the 16 lanes
+// that read one fragment column together fall on different banks:
+//   [OUT][BK]            chunk c of row o sits at c ^ (o & 7)
+//   [BK][OUT] 16-bit     32-byte unit u of row k at u ^ ((k & 3) | (k >> 3 & 1) << 2)
+//   [BK][OUT] float32    64-byte unit u of row k at u ^ (k >> 2 & 3)
+// Chunk L (row-major) of the tile is fetched by lane L, so the LDS side is linear, as LDS-DMA wants it, and the
+// permutation is on the memory side, inside lines that are fetched whole anyway.
+template <int DT, int TR, int OUT, int NT>
+struct Tile {
+    static constexpr int E = elem_size(DT);
+    static constexpr int BK = 128 / E;
+    static constexpr int BYTES = OUT * 128;
+    static constexpr int CH = BYTES / 16 / NT;                  // chunks per thread
+    static constexpr int CE = 16 / E;                           // elements per chunk
+    static constexpr int ROWC = TR ? OUT * E / 16 : 8;          // chunks per row
+    static constexpr int ROWB = ROWC * 16;
+    static_assert(BYTES % (16 * NT) == 0, "whole chunks per thread");
+
+    __device__ __forceinline__ static int row_of(int L) { return L / ROWC; }
+    // first element of chunk L within its row
+    __device__ __forceinline__ static int col_of(int L) {
+        const int row = L / ROWC, slot = L % ROWC;
+        if constexpr (!TR) return (slot ^ (row & 7)) * CE;
+        else if constexpr (E == 2) {
+            const int f = ((row & 3) | ((row >> 3 & 1) << 2)) & (OUT / 16 - 1);
+            return (((slot >> 1) ^ f) << 4) + (slot & 1) * 8;
+        } else {
+            const int f = (row >> 2 & 3) & (OUT / 16 - 1);
+            return (((slot >> 2) ^ f) << 4) + (slot & 3) * 4;
+        }
+    }
+    // fragment: lane (i = lane % 16, g = lane / 16) holds outer index o0 + i and reduction elements
+    // (4 s + g) CE .. + CE of the tile (s = 0, 1)
+    __device__ __forceinline__ static i32x4 frag(const unsigned char* tile, int o0, int s, int lane) {
+        const int i = lane & 15, g = lane >> 4;
+        if constexpr (!TR) {
+            return *reinterpret_cast<const i32x4*>(tile + (o0 + i) * 128 + (((4 * s + g) ^ (i & 7)) << 4));
+        } else if constexpr (E == 2) {
+            const int f = ((i >> 2) | ((g & 1) << 2)) & (OUT / 16 - 1);
+            const int k = s * 32 + g * 8 + (i >> 2);
+            const unsigned char* a = tile + k * ROWB + (((o0 >> 4) ^ f) << 5) + (i & 3) * 8;
+            typedef __attribute__((address_space(3))) s16x4* lds4;
+            union { s16x4 h[2]; i32x4 v; } u;
+            u.h[0] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(a));
+            u.h[1] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds4)(a + 4 * ROWB));
+            return u.v;
+        } else {
+            const int f = g & (OUT / 16 - 1);
+            const int k = s * 16 + g * 4;
+            const unsigned char* a = tile + k * ROWB + (((o0 >> 4) ^ f) << 6) + i * 4;
+            i32x4 v;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) v[j] = *reinterpret_cast<const int*>(a + j * ROWB);
+            return v;
+        }
+    }
+};
+
+template <int DT>
+__device__ __forceinline__ void mma(f32x4& c, const i32x4& a, const i32x4& b) {
+    if constexpr (DT == BF16)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8, a), __builtin_bit_cast(bf16x8, b), c, 0, 0, 0);
+    else if constexpr (DT == F16)
+        c = __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8, a), __builtin_bit_cast(f16x8, b), c, 0, 0, 0);
+    else if constexpr (DT == F32) {
+        const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
+#pragma unroll
+        for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
+    }
+}
+__device__ __forceinline__ void mma8(f32x4& c, const i32x4 (&a)[2], const i32x4 (&b)[2]) {
+    i32x8 x, y;
+#pragma unroll
+    for (int j = 0; j < 4; ++j) { x[j] = a[0][j]; x[4 + j] = a[1][j]; y[j] = b[0][j]; y[4 + j] = b[1][j]; }
+    // scale operands 0: the products enter unscaled
+    c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+}
+
+// LDS-DMA of 16 bytes per lane to lds .. lds + 1024: written as asm because hipcc, once it sees such a load, waits for
+// all of them before any LDS read.  A lane whose offset is not below the buffer's 2^31 - 1 bytes gets zeros.
+constexpr unsigned OUTSIDE = 0x80000000u;
+__device__ __forceinline__ i32x4 buffer_of(const void* p) {
+    const unsigned long long a = reinterpret_cast<unsigned long long>(p);
+    i32x4 r;
+    r[0] = __builtin_amdgcn_readfirstlane((int)(unsigned)a);
+    r[1] = __builtin_amdgcn_readfirstlane((int)(unsigned)(a >> 32)) & 0xffff;
+    r[2] = 0x7fffffff;
+    r[3] = 0x00020000;
+    return r;
+}
+__device__ __forceinline__ void dma16(unsigned lds, unsigned voff, const i32x4& rsrc) {
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+}
+
+// One operand's side of the main loop.
+template <int DT, int TR, int OUT, int NT, bool DMA>
+struct Loader {
+    using T = Tile<DT, TR, OUT, NT>;
+    uint4 st[DMA ? 1 : T::CH];
+
+    // base: the operand's first element of this tile of C and k-tile; outs / reds: how many rows of C and reduction
+    // elements are left from there
+    __device__ __forceinline__ void fetch(const char* base, long long ld, long long outs, long long reds, int tid, unsigned lds) {
+        if constexpr (DMA) {
+            const i32x4 rsrc = buffer_of(base);
+            const unsigned w = __builtin_amdgcn_readfirstlane(tid >> 6);
+            const int no = (int)(outs < OUT ? outs : OUT), nr = (int)(reds < T::BK ? reds : T::BK);
+#pragma unroll
+            for (int i = 0; i < T::CH; ++i) {
+                const int L = i * NT + tid;
+                const int row = T::row_of(L), col = T::col_of(L);
+                const bool in = TR ? (row < nr && col < no) : (row < no && col < nr);
+                const unsigned off = in ? (unsigned)(row * (int)ld + col) * T::E : OUTSIDE;
+                dma16(lds + (unsigned)(i * NT + w * 64) * 16, off, rsrc);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < T::CH; ++i) {
+                const int L = i * NT + tid;
+                const int row = T::row_of(L), col = T::col_of(L);
+                const long long rows = TR ? reds : outs, cols = TR ? outs : reds;
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (row < rows && col < cols) {
+                    const char* p = base + (row * ld + col) * T::E;
+                    const long long have = cols - col;
+                    if (have >= T::CE) __builtin_memcpy(&v, p, 16);      // any alignment: global loads take it
+                    else {
+                        unsigned w[4] = {0, 0, 0, 0};
+#pragma unroll
+                        for (int j = 0; j < T::CE - 1; ++j) {
+                            if (j < have) {
+                                if constexpr (T::E == 4) w[j] = reinterpret_cast<const unsigned*>(p)[j];
+                                else if constexpr (T::E == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
+                                else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
+                            }
+                        }
+                        v = make_uint4(w[0], w[1], w[2], w[3]);
+                    }
+                }
+                st[i] = v;
+            }
+        }
+    }
+    __device__ __forceinline__ void put(unsigned char* tile, int tid) {
+        if constexpr (!DMA) {
+#pragma unroll
+            for (int i = 0; i < T::CH; ++i) *reinterpret_cast<uint4*>(tile + (i * NT + tid) * 16) = st[i];
+        }
+    }
+};
+
+template <int WP, int WQ>
+__host__ __device__ constexpr int epi_bytes() { return 16 * (WQ + 4) * 4; }
+
+// BP x BQ of C per workgroup of WVP x WVQ waves.
+template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, bool DMA>
+__global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
+    constexpr int NT = WVP * WVQ * 64;
+    constexpr int TA = LAY == DW, TB = LAY != FWD;
+    constexpr int WP = BP / WVP, WQ = BQ / WVQ, FP = WP / 16, FQ = WQ / 16;
+    using LA = Loader<DT, TA, BP, NT, DMA>;
+    using LB = Loader<DT, TB, BQ, NT, DMA>;
+    using TAt = typename LA::T;
+    using TBt = typename LB::T;
+    constexpr int BK = TAt::BK, E = TAt::E;
+    constexpr int STAGE = TAt::BYTES + TBt::BYTES;
+    constexpr int EPI = WVP * WVQ * epi_bytes<WP, WQ>(), LDS = 2 * STAGE > EPI ? 2 * STAGE : EPI;
+    static_assert(LDS <= 160 * 1024, "LDS of one compute unit");
+    __shared__ __align__(1024) unsigned char smem[LDS];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int wp = (wave / WVQ) * WP, wq = (wave % WVQ) * WQ;
+
+    // workgroup -> tile: consecutive workgroups go to the 8 XCDs in turn, so XCD x takes the x-th eighth of the tiles,
+    // and within it walks 8 rows of tiles column by column: its L2 then holds both operands' panels
+    const unsigned n_tiles = g.tiles_p * g.tiles_q;
+    unsigned t = blockIdx.x;
+    {
+        const unsigned x = t & 7, i = t >> 3, each = n_tiles >> 3, more = n_tiles & 7;
+        t = x * each + (x < more ? x : more) + i;
+    }
+    const unsigned per = 8 * g.tiles_q, grp = t / per, first = grp * 8;
+    const unsigned rows = g.tiles_p - first < 8 ? g.tiles_p - first : 8, in = t - grp * per;
+    const long long p0 = (long long)(first + in % rows) * BP, q0 = (long long)(in / rows) * BQ;
+
+    const long long r_lo = g.splits > 1 ? (long long)blockIdx.y * g.red_part : 0;
+    long long red[2] = {g.seg[0].red, g.nseg > 1 ? g.seg[1].red : 0};
+    if (g.splits > 1) red[0] = red[0] - r_lo < g.red_part ? red[0] - r_lo : g.red_part;
+    const int nt0 = (int)((red[0] + BK - 1) / BK), nt = nt0 + (int)((red[1] + BK - 1) / BK);
+
+    LA la;
+    LB lb;
+    const unsigned lds0 = (unsigned)(unsigned long long)(lds_u8*)smem;
+    auto fetch = [&](int kt, int buf) {
+        const int s = kt >= nt0;
+        const Seg& sg = g.seg[s];
+        const long long r = (long long)(s ? kt - nt0 : kt) * BK, left = red[s] - r, ra = r_lo + r;
+        const char* pa = reinterpret_cast<const char*>(sg.a) + (TA ? ra * sg.lda + p0 : p0 * sg.lda + ra) * E;
+        const char* pb = reinterpret_cast<const char*>(sg.b) + (TB ? ra * sg.ldb + q0 : q0 * sg.ldb + ra) * E;
+        la.fetch(pa, sg.lda, g.P - p0, left, tid, lds0 + buf * STAGE);
+        lb.fetch(pb, sg.ldb, g.Q - q0, left, tid, lds0 + buf * STAGE + TAt::BYTES);
+    };
+    auto put = [&](int buf) {
+        la.put(smem + buf * STAGE, tid);
+        lb.put(smem + buf * STAGE + TAt::BYTES, tid);
+    };
+
+    f32x4 acc[FP][FQ];
+#pragma unroll
+    for (int i = 0; i < FP; ++i)
+#pragma unroll
+        for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+
+    if (nt > 0) fetch(0, 0);
+    put(0);
+    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    for (int kt = 0; kt < nt; ++kt) {
+        const int buf = kt & 1;
+        if (kt + 1 < nt) fetch(kt + 1, buf ^ 1);
+        const unsigned char* ta = smem + buf * STAGE;
+        const unsigned char* tb = ta + TAt::BYTES;
+        if constexpr (DT == F8) {
+            i32x4 b[FQ][2];
+#pragma unroll
+            for (int j = 0; j < FQ; ++j)
+#pragma unroll
+                for (int s = 0; s < 2; ++s) b[j][s] = TBt::frag(tb, wq + j * 16, s, lane);
+#pragma unroll
+            for (int i = 0; i < FP; ++i) {
+                i32x4 a[2];
+#pragma unroll
+                for (int s = 0; s < 2; ++s) a[s] = TAt::frag(ta, wp + i * 16, s, lane);
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) mma8(acc[i][j], b[j], a);
+            }
+        } else {
+#pragma unroll
+            for (int s = 0; s < 2; ++s) {
+                i32x4 b[FQ];
+#pragma unroll
+                for (int j = 0; j < FQ; ++j) b[j] = TBt::frag(tb, wq + j * 16, s, lane);
+#pragma unroll
+                for (int i = 0; i < FP; ++i) {
+                    const i32x4 a = TAt::frag(ta, wp + i * 16, s, lane);
+#pragma unroll
+                    for (int j = 0; j < FQ; ++j) mma<DT>(acc[i][j], b[j], a);
+                }
+            }
+        }
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        if constexpr (!DMA) { if (kt + 1 < nt) put(buf ^ 1); }
+        __syncthreads();
+    }
+
+    // The accumulator holds four columns of one row of C per lane and fragment; through 16 x WQ floats of LDS per wave
+    // it turns into eight columns per lane, whole lines per row, for the epilogue's reads and stores.
+    float* slab = reinterpret_cast<float*>(smem) + wave * (epi_bytes<WP, WQ>() / 4);
+    constexpr int LPR = WQ / 8, RPP = 64 / LPR;
+#pragma unroll
+    for (int i = 0; i < FP; ++i) {
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int j = 0; j < FQ; ++j)
+            *reinterpret_cast<f32x4*>(slab + (lane & 15) * (WQ + 4) + j * 16 + (lane >> 4) * 4) = acc[i][j];
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int r = 0; r < 16; r += RPP) {
+            const int row = r + lane / LPR, col = (lane % LPR) * 8;
+            if (RPP > 16 && row >= 16) continue;
+            const long long p = p0 + wp + i * 16 + row, q = q0 + wq + col;
+            float v[8];
+            const f32x4 lo = *reinterpret_cast<const f32x4*>(slab + row * (WQ + 4) + col);
+            const f32x4 hi = *reinterpret_cast<const f32x4*>(slab + row * (WQ + 4) + col + 4);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
+            if (p < g.P && q < g.Q) {
+                if (g.partial) {
+                    float* o = g.partial + ((long long)blockIdx.y * g.P + p) * g.Q + q;
+                    if (q + 8 <= g.Q) __builtin_memcpy(o, v, 32);
+                    else {
+#pragma unroll
+                        for (int j = 0; j < 8; ++j) if (q + j < g.Q) o[j] = v[j];
+                    }
+                } else epilogue8<DT>(g, p, q, v);
+            }
+        }
+    }
+}
+
+template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, bool DMA>
+int launch(GemmArgs& g, hipStream_t s) {
+    const long long tp = (g.P + BP - 1) / BP, tq = (g.Q + BQ - 1) / BQ;
+    NERF_REQUIRE(tp * tq < (1ll << 31), "linear: %lld x %lld outputs are too many for one launch", g.P, g.Q);
+    g.tiles_p = (unsigned)tp;
+    g.tiles_q = (unsigned)tq;
+    auto k = gemm_kernel<DT, LAY, BP, BQ, WVP, WVQ, DMA>;
+    hipLaunchKernelGGL(k, dim3((unsigned)(tp * tq), g.splits), dim3(WVP * WVQ * 64), 0, s, g);
+    NERF_LAUNCH_CHECK();
+    return NERF_OK;
+}
+
+}  // namespace lin
+}  // namespace nerf

@@ -15,8 +15,8 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NERF_HIP_LIB") or os.path.join(_HERE, "lib", "libnerf_hip.so")
 
 PREC_F32, PREC_BF16, PREC_BF16X3, PREC_BF16X2 = 0, 1, 2, 3
-ABI_VERSION = 7      # 2: training entry points take a precision; 3: nerf_mlp_backward_static; 4: nerf_mlp_forward_objects;
-                     # 5: nerf_make_rays_views; 6: the bf16x3 / bf16x2 precision codes
+ABI_VERSION = 8      # 2: training entry points take a precision; 3: nerf_mlp_backward_static; 4: nerf_mlp_forward_objects;
+                     # 5: nerf_make_rays_views; 6: the bf16x3 / bf16x2 precision codes; 8: layer operators
 IN_FEATURES, IN_POINTS, IN_RAYS = 0, 1, 2
 PRECISIONS = {"fp32": PREC_F32, "f32": PREC_F32, "float32": PREC_F32, "bf16": PREC_BF16, "bfloat16": PREC_BF16,
               # float32-accurate on the bf16 matrix cores: operands as sums of three (two) bf16 terms
@@ -94,6 +94,32 @@ _SIGNATURES = {
                                       ctypes.POINTER(ctypes.c_longlong), ctypes.c_longlong, ctypes.c_float,
                                       ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                       ctypes.c_void_p]),
+    "nerf_linear": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
+                                   ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                   ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
+                                   ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]),
+    "nerf_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+                                                               ctypes.c_int, ctypes.c_int]),
+    "nerf_linear_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
+                                            ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
+                                            ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                            ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                            ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
+                                            ctypes.c_void_p]),
+    "nerf_linear_q8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_longlong, _c_float_p, ctypes.c_void_p, ctypes.c_longlong,
+                                      _c_float_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
+                                      ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int,
+                                      ctypes.c_int, ctypes.c_void_p]),
+    "nerf_add_rms_norm": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
+                                         ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                         ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, _c_float_p, _c_float_p,
+                                         ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]),
+    "nerf_add_rms_norm_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_longlong, ctypes.c_int]),
+    "nerf_add_rms_norm_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                                  ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                                  _c_float_p, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
+                                                  ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
+                                                  ctypes.c_void_p]),
 }
 
 _lib = None
@@ -641,3 +667,173 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
             _check(lib().nerf_adam_step(k, mk(ps), mk(gs), mk(ms), mk(vs), numel, int(step), float(lr), float(beta1),
                                         float(beta2), float(eps), float(weight_decay), _stream(ps[0])), "nerf_adam_step")
     WEIGHT_GENERATION[0] += 1
+
+
+# --------------------------------------------------------------------------- layer operators
+DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
+NORM_MAX_WIDTH = 32768
+
+
+def activation_code(name):
+    if name not in ACTIVATIONS:
+        raise ValueError("unknown activation %r (one of %s)" % (name, ", ".join(repr(k) for k in ACTIVATIONS)))
+    return ACTIVATIONS[name]
+
+
+def _matrix(t, name, rows=None, cols=None, dtype=None, device=None):
+    """A [rows, cols] device matrix as the layer kernels take it: columns contiguous, any row stride of at least its row's
+    length.  Other layouts (transposed, expanded rows) are copied.  Returns (tensor, row stride)."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if not t.is_cuda:
+        raise ValueError("%s must live on a GPU (got %s); this engine has no CPU path" % (name, t.device))
+    if device is not None and t.device != device:
+        raise ValueError("%s is on %s but %s was expected" % (name, t.device, device))
+    if t.dtype != dtype and dtype is not None:
+        raise ValueError("%s must be %s like the input, got %s" % (name, dtype, t.dtype))
+    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
+        raise ValueError("%s must be [%s, %s], got %s" % (name, "n" if rows is None else rows, "n" if cols is None else cols, tuple(t.shape)))
+    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+        t = t.contiguous()
+    return t, max(t.stride(0), t.shape[1])
+
+
+def _vector(t, name, n, dtype, device):
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if not t.is_cuda or t.device != device or t.dtype != dtype or tuple(t.shape) != (n,):
+        raise ValueError("%s must be %s [%d] on %s, got %s %s on %s" % (name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _layer_dtype(t, name):
+    if isinstance(t, torch.Tensor) and t.dtype not in DTYPES:
+        raise ValueError("%s must be float32, bfloat16 or float16, got %s" % (name, t.dtype))
+
+
+def _layer_input(x0, x1, weight):
+    _layer_dtype(x0, "x")
+    x0, ld0 = _matrix(x0, "x")
+    M, k0 = x0.shape
+    ld1, k1 = 0, 0
+    if x1 is not None:
+        x1, ld1 = _matrix(x1, "the second piece of x", rows=M, dtype=x0.dtype, device=x0.device)
+        k1 = x1.shape[1]
+        _need(k1 >= 1, "the second piece of x has no columns")
+    _need(k0 >= 1, "x has no columns")
+    w, ldw = _matrix(weight, "weight", cols=k0 + k1, dtype=x0.dtype, device=x0.device)
+    _need(w.shape[0] >= 1, "weight has no rows")
+    return x0, ld0, k0, x1, ld1, k1, w, ldw
+
+
+def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_z=False):
+    """act([x0 | x1] weight^T + bias) + residual on matrices [M, k0], [M, k1], [N, k0 + k1], [N], [M, N] of one type.
+    Returns (y, z): z is the argument of act with want_z, else None."""
+    act = activation_code(activation)
+    x0, ld0, k0, x1, ld1, k1, w, ldw = _layer_input(x0, x1, weight)
+    M, N, dt, dev = x0.shape[0], w.shape[0], x0.dtype, x0.device
+    b = None if bias is None else _vector(bias, "bias", N, dt, dev)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)
+    y = torch.empty((M, N), dtype=dt, device=dev)
+    z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
+    with torch.cuda.device(dev):
+        _check(lib().nerf_linear(DTYPES[dt], _ptr(x0), ld0, k0, _ptr(x1), ld1, k1, _ptr(w), ldw, _ptr(b), act, _ptr(r), ldr,
+                                 _ptr(y), N, _ptr(z), N, M, N, _stream(y)), "nerf_linear")
+    return y, z
+
+
+def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=True, want_x1=True, want_w=True, want_b=True):
+    """Gradients of linear for g = dL/dy: (dx0, dx1, dweight, dbias), None where not wanted.  z: the argument of act that
+    the forward gave (for relu without a residual, y)."""
+    act = activation_code(activation)
+    x0, ld0, k0, x1, ld1, k1, w, ldw = _layer_input(x0, x1, weight)
+    M, N, dt, dev = x0.shape[0], w.shape[0], x0.dtype, x0.device
+    g, ldg = _matrix(g, "the gradient of y", M, N, dt, dev)
+    _need(act == 0 or z is not None, "linear_backward: the gradient through %s needs z", activation)
+    zz, ldz = (None, 0) if act == 0 else _matrix(z, "z", M, N, dt, dev)
+    new = lambda *shape: torch.empty(shape, dtype=dt, device=dev)
+    dx0 = new(M, k0) if want_x0 else None
+    dx1 = new(M, k1) if want_x1 and x1 is not None else None
+    dw = new(N, k0 + k1) if want_w else None
+    db = new(N) if want_b else None
+    nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], M, N, k0, k1, act)
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)      # its own in every call: calls on other streams may overlap
+    with torch.cuda.device(dev):
+        _check(lib().nerf_linear_backward(DTYPES[dt], _ptr(g), ldg, _ptr(zz), ldz, act, _ptr(x0), ld0, k0, _ptr(x1), ld1, k1,
+                                          _ptr(w), ldw, _ptr(dx0), k0, _ptr(dx1), k1, _ptr(dw), _ptr(db), M, N, _ptr(ws),
+                                          nbytes, _stream(g)), "nerf_linear_backward")
+    return dx0, dx1, dw, db
+
+
+def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
+    """act(x_scale w_scale (xq wq^T) + bias) + residual: xq [M, K] and wq [N, K] float8_e4m3fn with a float32 scale per
+    row; bias [N], residual [M, N] and the result of out_dtype."""
+    act = activation_code(activation)
+    _need(out_dtype in DTYPES, "linear_q8: out_dtype must be float32, bfloat16 or float16, got %s", out_dtype)
+    f8 = torch.float8_e4m3fn
+    _need(isinstance(xq, torch.Tensor) and xq.dtype == f8, "xq must be float8_e4m3fn, got %s",
+          xq.dtype if isinstance(xq, torch.Tensor) else type(xq).__name__)
+    xq, ldx = _matrix(xq, "xq")
+    M, K = xq.shape
+    dev = xq.device
+    _need(K >= 1, "xq has no columns")
+    wq, ldw = _matrix(wq, "wq", cols=K, dtype=f8, device=dev)
+    N = wq.shape[0]
+    _need(N >= 1, "wq has no rows")
+    xs = _vector(x_scale, "x_scale", M, torch.float32, dev)
+    ws = _vector(w_scale, "w_scale", N, torch.float32, dev)
+    b = None if bias is None else _vector(bias, "bias", N, out_dtype, dev)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_dtype, dev)
+    y = torch.empty((M, N), dtype=out_dtype, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().nerf_linear_q8(_ptr(xq), ldx, _ptr(xs), _ptr(wq), ldw, _ptr(ws), DTYPES[out_dtype], _ptr(b), act, _ptr(r),
+                                    ldr, _ptr(y), N, M, N, K, _stream(y)), "nerf_linear_q8")
+    return y
+
+
+def _norm_input(x, weight, residual):
+    _layer_dtype(x, "x")
+    x, ldx = _matrix(x, "x")
+    M, N = x.shape
+    _need(1 <= N <= NORM_MAX_WIDTH, "add_rms_norm: rows of 1 to %d columns, got %d", NORM_MAX_WIDTH, N)
+    w = _vector(weight, "weight", N, x.dtype, x.device)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, x.dtype, x.device)
+    return x, ldx, M, N, w, r, ldr
+
+
+def add_rms_norm(x, weight, residual=None, eps=1e-6, want_h=True, want_rstd=False, q8=False):
+    """h = x + residual, y = weight h / sqrt(mean(h^2) + eps) on matrices [M, N].  Returns (y, h, rstd), or with q8
+    (q, scale, h): q float8_e4m3fn [M, N], scale float32 [M].  h and rstd are None where not wanted."""
+    x, ldx, M, N, w, r, ldr = _norm_input(x, weight, residual)
+    dt, dev = x.dtype, x.device
+    _need(float(eps) >= 0.0, "add_rms_norm: eps must not be negative, got %s", eps)
+    h = torch.empty((M, N), dtype=dt, device=dev) if want_h else None
+    y = None if q8 else torch.empty((M, N), dtype=dt, device=dev)
+    q = torch.empty((M, N), dtype=torch.float8_e4m3fn, device=dev) if q8 else None
+    scale = torch.empty((M,), dtype=torch.float32, device=dev) if q8 else None
+    rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
+    with torch.cuda.device(dev):
+        _check(lib().nerf_add_rms_norm(DTYPES[dt], _ptr(x), ldx, _ptr(r), ldr, _ptr(w), float(eps), _ptr(h), N, _ptr(y), N,
+                                       _ptr(q), N, _ptr(scale), _ptr(rstd), M, N, _stream(x)), "nerf_add_rms_norm")
+    return (q, scale, h) if q8 else (y, h, rstd)
+
+
+def add_rms_norm_backward(gy, h, weight, rstd, gh=None, want_x=True, want_w=True):
+    """(dx, dweight) of add_rms_norm for gy = dL/dy and gh = dL/dh; dx is the residual's gradient too."""
+    h, ldh, M, N, w, _, _ = _norm_input(h, weight, None)
+    dt, dev = h.dtype, h.device
+    gy, ldgy = _matrix(gy, "the gradient of y", M, N, dt, dev)
+    gh, ldgh = (None, 0) if gh is None else _matrix(gh, "the gradient of h", M, N, dt, dev)
+    rstd = _vector(rstd, "rstd", M, torch.float32, dev)
+    dx = torch.empty((M, N), dtype=dt, device=dev) if want_x else None
+    dw = torch.empty((N,), dtype=dt, device=dev) if want_w else None
+    if dx is None and dw is None:
+        return None, None
+    nbytes = lib().nerf_add_rms_norm_backward_workspace_bytes(M, N) if want_w else 0
+    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
+    with torch.cuda.device(dev):
+        _check(lib().nerf_add_rms_norm_backward(DTYPES[dt], _ptr(gy), ldgy, _ptr(gh), ldgh, _ptr(h), ldh, _ptr(w), _ptr(rstd),
+                                                _ptr(dx), N, _ptr(dw), M, N, _ptr(ws), nbytes, _stream(h)),
+               "nerf_add_rms_norm_backward")
+    return dx, dw

@@ -1,0 +1,159 @@
+"""Layers of networks of any shape as single kernels, with gradients: what NeRF evaluates layer by layer when the fused
+renderer kernels do not cover it (other depths and widths, residual trunks), usable on their own.
+
+  linear(x, weight, bias, activation, residual)   act(x W^T + b) + r; x may be two pieces side by side (a skip connection)
+  add_rms_norm(x, weight, residual)               the residual addition and the root-mean-square norm behind it
+  add_rms_norm_q8(x, weight, residual)            the same with an 8-bit output and one scale a row
+  linear_q8(xq, x_scale, wq, w_scale, ...)        the linear layer on such operands
+  quantize_weight(weight)                         a weight matrix as (wq, w_scale)
+
+Tensors live on one GPU and share one type (float32, bfloat16, float16); sums, norms and scales are float32.  Leading
+dimensions are free.  The kernels run on the current stream of the tensors' device, allocate nothing but their results
+and scratch through torch, and can be captured in a graph.  Gradients are computed once (no second derivatives), and
+torch.autocast does not change the types here.
+"""
+import torch
+from torch.autograd.function import once_differentiable
+
+from . import hip
+
+
+def _flat(t, name):
+    """[..., n] -> [m, n] without a copy where the layout allows it."""
+    if not isinstance(t, torch.Tensor):
+        raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+    if t.dim() < 1:
+        raise ValueError("%s must have at least one dimension" % name)
+    return t if t.dim() == 2 else t.reshape(t.shape[:-1].numel(), t.shape[-1])
+
+
+class _LinearFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x0, x1, weight, bias, residual, activation):
+        needs = ctx.needs_input_grad
+        inner = any(needs[:4])
+        # relu without a residual: y > 0 is where its argument is, so y stands in for it
+        own = activation == "relu" and residual is None
+        y, z = hip.linear(x0, weight, bias, activation, residual, x1,
+                          want_z=inner and not own and hip.activation_code(activation) != 0)
+        ctx.activation = activation
+        ctx.bias = bias is not None
+        # x is read by the weight's gradient, the weight by x's
+        ctx.save_for_backward(x0 if inner else None, x1 if inner else None, weight if inner else None, y if own and inner else z)
+        return y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy):
+        x0, x1, weight, z = ctx.saved_tensors
+        n0, n1, nw, nb, nr, _ = ctx.needs_input_grad
+        dx0 = dx1 = dw = db = None
+        if n0 or n1 or nw or nb:
+            dx0, dx1, dw, db = hip.linear_backward(gy, x0, weight, z, ctx.activation, x1, n0, n1, nw, nb)
+        return dx0, dx1, dw, db, gy if nr else None, None
+
+
+def linear(x, weight, bias=None, activation=None, residual=None):
+    """act(x weight^T + bias) + residual in one launch, differentiable in every tensor.
+
+    x [..., K], or a pair ([..., K0], [..., K1]) that stands for their concatenation; weight [N, K] as nn.Linear holds it;
+    bias [N]; residual [..., N] (exactly the result's shape); activation None, "relu", "gelu" (the exact one) or "silu"."""
+    x0, x1 = x if isinstance(x, (tuple, list)) and len(x) == 2 else (x, None)
+    a = _flat(x0, "x")
+    lead = tuple(x0.shape[:-1])
+    b = None
+    if x1 is not None:
+        b = _flat(x1, "the second piece of x")
+        if tuple(x1.shape[:-1]) != lead:
+            raise ValueError("the pieces of x have leading shapes %s and %s" % (lead, tuple(x1.shape[:-1])))
+    r = None
+    if residual is not None:
+        r = _flat(residual, "residual")
+        if tuple(residual.shape[:-1]) != lead:
+            raise ValueError("residual has leading shape %s, x %s" % (tuple(residual.shape[:-1]), lead))
+    y = _LinearFn.apply(a, b, weight, bias, r, "none" if activation is None else activation)
+    return y if len(lead) == 1 else y.reshape(lead + (y.shape[-1],))
+
+
+class _AddNormFn(torch.autograd.Function):
+    """(y, h) with a residual, y alone without one (h is x then, and its gradient reaches x by itself)."""
+
+    @staticmethod
+    def forward(ctx, x, weight, residual, eps):
+        inner = any(ctx.needs_input_grad[:3])
+        y, h, rstd = hip.add_rms_norm(x, weight, residual, eps, want_h=residual is not None, want_rstd=inner)
+        ctx.two = residual is not None
+        if inner:
+            ctx.save_for_backward(h if ctx.two else x, weight, rstd)
+        ctx.set_materialize_grads(False)
+        return (y, h) if ctx.two else y
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, gy, gh=None):
+        nx, nw, nr, _ = ctx.needs_input_grad
+        if gy is None:
+            zero = None
+            if nw and gh is not None:
+                zero = torch.zeros_like(ctx.saved_tensors[1])
+            return gh if nx else None, zero, gh if nr else None, None
+        h, weight, rstd = ctx.saved_tensors
+        dx, dw = hip.add_rms_norm_backward(gy, h, weight, rstd, gh, want_x=nx or nr, want_w=nw)
+        return dx if nx else None, dw, dx if nr else None, None
+
+
+def add_rms_norm(x, weight, residual=None, eps=1e-6):
+    """h = x + residual and y = weight h / sqrt(mean(h^2) + eps) over the last dimension, in one pass.  Returns (y, h);
+    without a residual h is x itself.  Differentiable in x, weight and residual; at most 32768 columns.
+
+    In 16-bit types y comes from the float32 sum, h is that sum rounded, and the backward starts from the rounded h."""
+    a = _flat(x, "x")
+    if residual is None:
+        y = _AddNormFn.apply(a, weight, None, float(eps))
+        return y.reshape(x.shape), x
+    if tuple(residual.shape) != tuple(x.shape):
+        raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
+    y, h = _AddNormFn.apply(a, weight, _flat(residual, "residual"), float(eps))
+    return y.reshape(x.shape), h.reshape(x.shape)
+
+
+def _no_grad(what, *tensors):
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+        raise NotImplementedError("%s has no gradient (8-bit numbers are for inference): call it under torch.no_grad()" % what)
+
+
+def add_rms_norm_q8(x, weight, residual=None, eps=1e-6):
+    """add_rms_norm with y in 8 bits: returns (q, scale, h), q float8_e4m3fn like x and scale float32 [...], y = scale q.
+    scale = max(max|y| / 448, 2^-126) of its row; a row with an infinity or NaN reads back as NaN."""
+    _no_grad("add_rms_norm_q8", x, weight, residual)
+    a = _flat(x, "x")
+    r = None
+    if residual is not None:
+        if tuple(residual.shape) != tuple(x.shape):
+            raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
+        r = _flat(residual, "residual")
+    q, scale, h = hip.add_rms_norm(a, weight, r, eps, want_h=r is not None, q8=True)
+    return q.reshape(x.shape), scale.reshape(x.shape[:-1]), x if h is None else h.reshape(x.shape)
+
+
+def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
+    """act(x W^T + bias) + residual with x = x_scale xq (xq float8_e4m3fn [..., K], x_scale float32 [...]) and
+    W = w_scale wq ([N, K], [N]); bias, residual and the result are of out_dtype.  No gradient."""
+    _no_grad("linear_q8", x_scale, w_scale, bias, residual)
+    a = _flat(xq, "xq")
+    lead = tuple(xq.shape[:-1])
+    if not isinstance(x_scale, torch.Tensor) or tuple(x_scale.shape) != lead:
+        raise ValueError("x_scale must be a tensor of shape %s" % (lead,))
+    if residual is not None and tuple(residual.shape[:-1]) != lead:
+        raise ValueError("residual has leading shape %s, xq %s" % (tuple(residual.shape[:-1]), lead))
+    y = hip.linear_q8(a, x_scale.reshape(-1), wq, w_scale, bias, activation,
+                      None if residual is None else _flat(residual, "residual"), out_dtype)
+    return y if len(lead) == 1 else y.reshape(lead + (y.shape[-1],))
+
+
+@torch.no_grad()
+def quantize_weight(weight):
+    """(wq float8_e4m3fn [N, K], w_scale float32 [N]) for linear_q8, made once per weight version with torch."""
+    w = weight.float()
+    scale = (w.abs().amax(-1) / 448.0).clamp_min(2.0 ** -126)
+    return (w / scale[:, None]).to(torch.float8_e4m3fn), scale
