@@ -13,8 +13,10 @@
 namespace nerf {
 namespace lin {
 
-enum { F32 = NERF_DT_F32, BF16 = NERF_DT_BF16, F16 = NERF_DT_F16, F8 = 3 };
-constexpr int elem_size(int dt) { return dt == F32 ? 4 : dt == F8 ? 1 : 2; }
+// F8: e4m3 operands on the 8-bit matrix instructions; F8W: the same operands widened to bf16 first (exact), see mma8w
+enum { F32 = NERF_DT_F32, BF16 = NERF_DT_BF16, F16 = NERF_DT_F16, F8 = 3, F8W = 4 };
+constexpr bool is_f8(int dt) { return dt >= F8; }
+constexpr int elem_size(int dt) { return dt == F32 ? 4 : is_f8(dt) ? 1 : 2; }
 
 typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef int i32x4 __attribute__((ext_vector_type(4)));
@@ -58,6 +60,8 @@ int gemm_f32(int layout, GemmArgs& g, hipStream_t s);
 int gemm_bf16(int layout, GemmArgs& g, hipStream_t s);
 int gemm_f16(int layout, GemmArgs& g, hipStream_t s);
 int gemm_f8(GemmArgs& g, hipStream_t s);
+// out [rows, cols] (rows ldo apart) = sum over n parts [rows][cols], in a fixed order (linear.hip)
+int part_sum(int dtype, const float* parts, int n, long long rows, long long cols, void* out, long long ldo, hipStream_t s);
 
 // ---------------------------------------------------------------------------------------------- scalars and epilogue
 __device__ __forceinline__ float ld_elem(const void* p, long long i, int dt) {
@@ -158,14 +162,14 @@ __device__ __forceinline__ float act_grad(float z, int act) {
 // the epilogue's types: of the operands, or, for 8-bit operands, named by the call
 template <int DT>
 __device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8], int dt) {
-    if constexpr (DT != F8) ld8<DT>(p, i, v);
+    if constexpr (!is_f8(DT)) ld8<DT>(p, i, v);
     else if (dt == F32) ld8<F32>(p, i, v);
     else if (dt == BF16) ld8<BF16>(p, i, v);
     else ld8<F16>(p, i, v);
 }
 template <int DT>
 __device__ __forceinline__ void store8(void* p, long long i, const float (&v)[8], int dt) {
-    if constexpr (DT != F8) st8<DT>(p, i, v);
+    if constexpr (!is_f8(DT)) st8<DT>(p, i, v);
     else if (dt == F32) st8<F32>(p, i, v);
     else if (dt == BF16) st8<BF16>(p, i, v);
     else st8<F16>(p, i, v);
@@ -178,7 +182,7 @@ __device__ __forceinline__ void some8(const void* p, long long i, bool whole, in
     if (whole) load8<DT>(p, i, v, dt);
     else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? ld_elem(p, i + j, DT == F8 ? dt : DT) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? ld_elem(p, i + j, is_f8(DT) ? dt : DT) : 0.f;
     }
 }
 template <int DT>
@@ -186,7 +190,7 @@ __device__ __forceinline__ void put_some8(void* p, long long i, bool whole, int 
     if (whole) store8<DT>(p, i, v, dt);
     else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) st_elem(p, i + j, v[j], DT == F8 ? dt : DT);
+        for (int j = 0; j < 8; ++j) if (j < n) st_elem(p, i + j, v[j], is_f8(DT) ? dt : DT);
     }
 }
 template <int DT>
@@ -194,7 +198,7 @@ __device__ __forceinline__ void epilogue8(const GemmArgs& g, long long p, long l
     const bool whole = q + 8 <= g.Q;
     const int n = whole ? 8 : (int)(g.Q - q);
     float t[8];
-    if constexpr (DT == F8) {
+    if constexpr (is_f8(DT)) {
         const float s = g.sp[p];
         some8<F32>(g.sq, q, whole, n, t, F32);
 #pragma unroll
@@ -284,6 +288,7 @@ struct Tile {
     }
 };
 
+__device__ __forceinline__ void mma8w(f32x4& c, const i32x4& a, const i32x4& b);
 template <int DT>
 __device__ __forceinline__ void mma(f32x4& c, const i32x4& a, const i32x4& b) {
     if constexpr (DT == BF16)
@@ -294,7 +299,7 @@ __device__ __forceinline__ void mma(f32x4& c, const i32x4& a, const i32x4& b) {
         const f32x4 x = __builtin_bit_cast(f32x4, a), y = __builtin_bit_cast(f32x4, b);
 #pragma unroll
         for (int j = 0; j < 4; ++j) c = __builtin_amdgcn_mfma_f32_16x16x4f32(x[j], y[j], c, 0, 0, 0);
-    }
+    } else if constexpr (DT == F8W) mma8w(c, a, b);
 }
 __device__ __forceinline__ void mma8(f32x4& c, const i32x4 (&a)[2], const i32x4 (&b)[2]) {
     i32x8 x, y;
@@ -302,6 +307,30 @@ __device__ __forceinline__ void mma8(f32x4& c, const i32x4 (&a)[2], const i32x4 
     for (int j = 0; j < 4; ++j) { x[j] = a[0][j]; x[4 + j] = a[1][j]; y[j] = b[0][j]; y[4 + j] = b[1][j]; }
     // scale operands 0: the products enter unscaled
     c = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(x, y, c, 0, 0, 0, 0, 0, 0);
+}
+
+// The 8-bit instruction adds its products in groups of eight at a resolution of 2^-13 of the group's largest, cutting
+// off what lies below (measured: a relative 1.4e-5 on rows of quantised normal numbers).  bf16 and fp16 results, rounded
+// to 2^-9 and 2^-12, do not show it; float32 results would, so theirs come from the bf16 instruction on the widened
+// numbers, at half the rate.
+__device__ __forceinline__ bf16x8 widen(unsigned lo, unsigned hi) {
+    unsigned o[4];
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+        const unsigned v = j ? hi : lo;
+        const f32x2 a = __builtin_amdgcn_cvt_pk_f32_fp8(v, false), b = __builtin_amdgcn_cvt_pk_f32_fp8(v, true);
+        const float a0 = a[0], a1 = a[1], b0 = b[0], b1 = b[1];     // scalars: a bit_cast of a vector's element takes its first
+        // every e4m3 number is a bf16 number: the upper halves of the floats
+        o[2 * j] = __builtin_amdgcn_perm(__float_as_uint(a1), __float_as_uint(a0), 0x07060302);
+        o[2 * j + 1] = __builtin_amdgcn_perm(__float_as_uint(b1), __float_as_uint(b0), 0x07060302);
+    }
+    bf16x8 r;
+    __builtin_memcpy(&r, o, 16);
+    return r;
+}
+__device__ __forceinline__ void mma8w(f32x4& c, const i32x4& a, const i32x4& b) {
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(a[0], a[1]), widen(b[0], b[1]), c, 0, 0, 0);
+    c = __builtin_amdgcn_mfma_f32_16x16x32_bf16(widen(a[2], a[3]), widen(b[2], b[3]), c, 0, 0, 0);
 }
 
 // LDS-DMA of 16 bytes per lane to lds .. lds + 1024: written as asm because hipcc, once it sees such a load, waits for
@@ -320,50 +349,73 @@ __device__ __forceinline__ void dma16(unsigned lds, unsigned voff, const i32x4& 
     asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
 }
 
-// One operand's side of the main loop.
+// The first `have` (1 .. CE - 1) elements at p, zeros behind them.  Not unrolled: it runs once at a row's end.
+template <int E>
+__device__ __forceinline__ uint4 part_chunk(const char* p, int have) {
+    unsigned long long lo = 0, hi = 0;
+#pragma unroll 1
+    for (int j = 0; j < have; ++j) {
+        const unsigned long long v = E == 4 ? reinterpret_cast<const unsigned*>(p)[j]
+                                   : E == 2 ? reinterpret_cast<const unsigned short*>(p)[j] : reinterpret_cast<const unsigned char*>(p)[j];
+        const int at = j * E;
+        if (at < 8) lo |= v << (8 * at);
+        else hi |= v << (8 * (at - 8));
+    }
+    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+}
+
+// One operand's side of the main loop.  A tile's chunks lie at fixed offsets from its first element, worked out once per
+// piece of the reduction; only a k-tile that runs over the reduction's end looks at every chunk again.
 template <int DT, int TR, int OUT, int NT, bool DMA>
 struct Loader {
     using T = Tile<DT, TR, OUT, NT>;
     uint4 st[DMA ? 1 : T::CH];
+    unsigned off[T::CH];         // bytes from the tile's first element
+    bool fast;                   // whole k-tiles need no check: rows are there (or doubled), chunks of outputs are whole
 
-    // base: the operand's first element of this tile of C and k-tile; outs / reds: how many rows of C and reduction
-    // elements are left from there
+    // outs: rows of C this operand has from the tile's first on
+    __device__ __forceinline__ void start(long long ld, long long outs, int tid) {
+        const int no = (int)(outs < OUT ? outs : OUT);
+        fast = DMA || ((!TR || no == OUT) && ld * T::E * 256 < (1ll << 31));
+#pragma unroll
+        for (int i = 0; i < T::CH; ++i) {
+            const int L = i * NT + tid;
+            const int row = T::row_of(L), col = T::col_of(L);
+            // rows behind the last: zeros by LDS-DMA; the last one again by loads (what they give is never stored)
+            if constexpr (DMA) off[i] = (TR ? col : row) < no ? (unsigned)(row * (int)ld + col) * T::E : OUTSIDE;
+            else off[i] = fast ? (unsigned)((TR || row < no ? row : no - 1) * (int)ld + col) * T::E : 0u;
+        }
+    }
+    // base: the tile's first element at this k-tile; reds: what is left of the reduction from there
     __device__ __forceinline__ void fetch(const char* base, long long ld, long long outs, long long reds, int tid, unsigned lds) {
         if constexpr (DMA) {
             const i32x4 rsrc = buffer_of(base);
-            const unsigned w = __builtin_amdgcn_readfirstlane(tid >> 6);
-            const int no = (int)(outs < OUT ? outs : OUT), nr = (int)(reds < T::BK ? reds : T::BK);
+            const unsigned at = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
+            if (reds >= T::BK) {
 #pragma unroll
-            for (int i = 0; i < T::CH; ++i) {
-                const int L = i * NT + tid;
-                const int row = T::row_of(L), col = T::col_of(L);
-                const bool in = TR ? (row < nr && col < no) : (row < no && col < nr);
-                const unsigned off = in ? (unsigned)(row * (int)ld + col) * T::E : OUTSIDE;
-                dma16(lds + (unsigned)(i * NT + w * 64) * 16, off, rsrc);
+                for (int i = 0; i < T::CH; ++i) dma16(at + i * NT * 16, off[i], rsrc);
+            } else {
+#pragma unroll
+                for (int i = 0; i < T::CH; ++i) {
+                    const int L = i * NT + tid;
+                    dma16(at + i * NT * 16, (TR ? T::row_of(L) : T::col_of(L)) < reds ? off[i] : OUTSIDE, rsrc);
+                }
             }
+        } else if (fast && reds >= T::BK) {
+#pragma unroll
+            for (int i = 0; i < T::CH; ++i) __builtin_memcpy(&st[i], base + off[i], 16);      // any alignment: global loads take it
         } else {
+            const long long rows = TR ? reds : outs, cols = TR ? outs : reds;
 #pragma unroll
             for (int i = 0; i < T::CH; ++i) {
                 const int L = i * NT + tid;
                 const int row = T::row_of(L), col = T::col_of(L);
-                const long long rows = TR ? reds : outs, cols = TR ? outs : reds;
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row < rows && col < cols) {
                     const char* p = base + (row * ld + col) * T::E;
                     const long long have = cols - col;
-                    if (have >= T::CE) __builtin_memcpy(&v, p, 16);      // any alignment: global loads take it
-                    else {
-                        unsigned w[4] = {0, 0, 0, 0};
-#pragma unroll
-                        for (int j = 0; j < T::CE - 1; ++j) {
-                            if (j < have) {
-                                if constexpr (T::E == 4) w[j] = reinterpret_cast<const unsigned*>(p)[j];
-                                else if constexpr (T::E == 2) w[j / 2] |= (unsigned)reinterpret_cast<const unsigned short*>(p)[j] << (16 * (j % 2));
-                                else w[j / 4] |= (unsigned)reinterpret_cast<const unsigned char*>(p)[j] << (8 * (j % 4));
-                            }
-                        }
-                        v = make_uint4(w[0], w[1], w[2], w[3]);
-                    }
+                    if (have >= T::CE) __builtin_memcpy(&v, p, 16);
+                    else v = part_chunk<T::E>(p, (int)have);
                 }
                 st[i] = v;
             }
@@ -421,12 +473,18 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     auto fetch = [&](int kt, int buf) {
         const int s = kt >= nt0;
         const Seg& sg = g.seg[s];
+        if (kt == nt0) {         // the second piece has a row stride of its own
+            la.start(sg.lda, g.P - p0, tid);
+            lb.start(sg.ldb, g.Q - q0, tid);
+        }
         const long long r = (long long)(s ? kt - nt0 : kt) * BK, left = red[s] - r, ra = r_lo + r;
         const char* pa = reinterpret_cast<const char*>(sg.a) + (TA ? ra * sg.lda + p0 : p0 * sg.lda + ra) * E;
         const char* pb = reinterpret_cast<const char*>(sg.b) + (TB ? ra * sg.ldb + q0 : q0 * sg.ldb + ra) * E;
         la.fetch(pa, sg.lda, g.P - p0, left, tid, lds0 + buf * STAGE);
         lb.fetch(pb, sg.ldb, g.Q - q0, left, tid, lds0 + buf * STAGE + TAt::BYTES);
     };
+    la.start(g.seg[0].lda, g.P - p0, tid);
+    lb.start(g.seg[0].ldb, g.Q - q0, tid);
     auto put = [&](int buf) {
         la.put(smem + buf * STAGE, tid);
         lb.put(smem + buf * STAGE + TAt::BYTES, tid);
@@ -438,16 +496,23 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
 #pragma unroll
         for (int j = 0; j < FQ; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
 
-    if (nt > 0) fetch(0, 0);
-    put(0);
-    if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __syncthreads();
-    for (int kt = 0; kt < nt; ++kt) {
-        const int buf = kt & 1;
-        if (kt + 1 < nt) fetch(kt + 1, buf ^ 1);
-        const unsigned char* ta = smem + buf * STAGE;
-        const unsigned char* tb = ta + TAt::BYTES;
-        if constexpr (DT == F8) {
+    // Two k-tiles are in LDS, and the fragments of the next half tile are on their way to registers while the matrix cores
+    // work on this one's: the one barrier of an iteration sits between the halves, where everything the second half needs
+    // has been read, so the tile's buffer is free for the k-tile after the next, and the next one's loads have had a whole
+    // iteration to land.
+    auto landed = [&] {
+        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+    };
+    if constexpr (DT == F8) {
+        fetch(0, 0);
+        put(0);
+        landed();
+        for (int kt = 0; kt < nt; ++kt) {
+            const int buf = kt & 1;
+            if (kt + 1 < nt) fetch(kt + 1, buf ^ 1);
+            const unsigned char* ta = smem + buf * STAGE;
+            const unsigned char* tb = ta + TAt::BYTES;
             i32x4 b[FQ][2];
 #pragma unroll
             for (int j = 0; j < FQ; ++j)
@@ -461,22 +526,54 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
 #pragma unroll
                 for (int j = 0; j < FQ; ++j) mma8(acc[i][j], b[j], a);
             }
-        } else {
+            if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            if constexpr (!DMA) { if (kt + 1 < nt) put(buf ^ 1); }
+            __syncthreads();
+        }
+    } else {
+        struct Half { i32x4 a[FP], b[FQ]; };
+        Half h0, h1;
+        auto read = [&](Half& h, int kt, int s) {
+            const unsigned char* ta = smem + (kt & 1) * STAGE;
+            const unsigned char* tb = ta + TAt::BYTES;
 #pragma unroll
-            for (int s = 0; s < 2; ++s) {
-                i32x4 b[FQ];
+            for (int j = 0; j < FQ; ++j) h.b[j] = TBt::frag(tb, wq + j * 16, s, lane);
 #pragma unroll
-                for (int j = 0; j < FQ; ++j) b[j] = TBt::frag(tb, wq + j * 16, s, lane);
+            for (int i = 0; i < FP; ++i) h.a[i] = TAt::frag(ta, wp + i * 16, s, lane);
+        };
+        auto work = [&](const Half& h) {
 #pragma unroll
-                for (int i = 0; i < FP; ++i) {
-                    const i32x4 a = TAt::frag(ta, wp + i * 16, s, lane);
+            for (int i = 0; i < FP; ++i)
 #pragma unroll
-                    for (int j = 0; j < FQ; ++j) mma<DT>(acc[i][j], b[j], a);
+                for (int j = 0; j < FQ; ++j) mma<DT>(acc[i][j], h.b[j], h.a[i]);
+        };
+        fetch(0, 0);
+        put(0);
+        if (nt > 1) {
+            fetch(1, 1);
+            put(1);
+        }
+        landed();
+        if constexpr (!DMA) { if (nt > 2) fetch(2, 0); }
+        read(h0, 0, 0);
+        for (int kt = 0; kt < nt; ++kt) {
+            read(h1, kt, 1);
+            __builtin_amdgcn_sched_barrier(0);
+            work(h0);
+            __builtin_amdgcn_sched_barrier(0);
+            landed();
+            if (kt + 2 < nt) {
+                if constexpr (DMA) fetch(kt + 2, kt & 1);
+                else {
+                    put(kt & 1);
+                    if (kt + 3 < nt) fetch(kt + 3, 0);
                 }
             }
+            if (kt + 1 < nt) read(h0, kt + 1, 0);
+            __builtin_amdgcn_sched_barrier(0);
+            work(h1);
+            __builtin_amdgcn_sched_barrier(0);
         }
-        if constexpr (DMA) asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-        if constexpr (!DMA) { if (kt + 1 < nt) put(buf ^ 1); }
         __syncthreads();
     }
 
@@ -525,6 +622,92 @@ int launch(GemmArgs& g, hipStream_t s) {
     g.tiles_q = (unsigned)tq;
     auto k = gemm_kernel<DT, LAY, BP, BQ, WVP, WVQ, DMA>;
     hipLaunchKernelGGL(k, dim3((unsigned)(tp * tq), g.splits), dim3(WVP * WVQ * 64), 0, s, g);
+    NERF_LAUNCH_CHECK();
+    return NERF_OK;
+}
+
+// ---------------------------------------------------------------------------------------------- few rows
+// One to 64 samples: every weight is read once and used a few times, so the time is the weights' way from memory.  A
+// workgroup owns 16 outputs; its NW waves take 64-byte steps of the reduction in turn (together whole lines of 16 weight
+// rows), straight from memory into fragments, U steps in flight each, and add their sums in LDS.
+template <int DT>
+__device__ __forceinline__ i32x4 chunk_at(const char* p, long long have) {
+    constexpr int E = elem_size(DT), CE = 16 / E;
+    i32x4 v = {0, 0, 0, 0};
+    if (have >= CE) __builtin_memcpy(&v, p, 16);
+    else if (have > 0) {
+        const uint4 t = part_chunk<E>(p, (int)have);
+        v = i32x4{(int)t.x, (int)t.y, (int)t.z, (int)t.w};
+    }
+    return v;
+}
+
+template <int DT, int MT, int NW>
+__global__ void __launch_bounds__(NW * 64) few_rows_kernel(const GemmArgs g) {
+    constexpr int E = elem_size(DT), CE = 16 / E, STEP = 4 * CE, U = (MT == 1 ? 8 : MT == 2 ? 4 : 2) / (DT == F8W ? 2 : 1);
+    __shared__ __align__(16) float sums[NW][MT][16][20];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, i = lane & 15, c = (lane >> 4) * CE;
+    const long long q0 = (long long)blockIdx.x * 16, q = q0 + i < g.Q ? q0 + i : g.Q - 1;
+    f32x4 acc[MT];
+#pragma unroll
+    for (int m = 0; m < MT; ++m) acc[m] = f32x4{0.f, 0.f, 0.f, 0.f};
+    int turn = 0;                // steps go round the waves across both pieces
+    for (int sgi = 0; sgi < g.nseg; ++sgi) {
+        const Seg& sg = g.seg[sgi];
+        const char* w = reinterpret_cast<const char*>(sg.b) + (q * sg.ldb + c) * E;
+        const char* x[MT];
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+            const long long p = m * 16 + i < g.P ? m * 16 + i : g.P - 1;     // rows behind the last repeat it
+            x[m] = reinterpret_cast<const char*>(sg.a) + (p * sg.lda + c) * E;
+        }
+        const int whole = (int)(sg.red / STEP), steps = (int)((sg.red + STEP - 1) / STEP);
+        int st = (wave - turn) & (NW - 1);
+        for (; st + (U - 1) * NW < whole; st += U * NW) {
+            i32x4 a[U], b[U][MT];
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const long long o = (long long)(st + u * NW) * 64;
+                __builtin_memcpy(&a[u], w + o, 16);
+#pragma unroll
+                for (int m = 0; m < MT; ++m) __builtin_memcpy(&b[u][m], x[m] + o, 16);
+            }
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int m = 0; m < MT; ++m) mma<DT>(acc[m], a[u], b[u][m]);
+                if constexpr (DT == F8W) __builtin_amdgcn_sched_barrier(0);      // widen one step at a time: registers
+            }
+        }
+        for (; st < steps; st += NW) {
+            const long long o = (long long)st * 64, have = sg.red - (long long)st * STEP - c;
+            const i32x4 a = chunk_at<DT>(w + o, have);
+#pragma unroll
+            for (int m = 0; m < MT; ++m) mma<DT>(acc[m], a, chunk_at<DT>(x[m] + o, have));
+        }
+        turn = (turn + steps) & (NW - 1);
+    }
+#pragma unroll
+    for (int m = 0; m < MT; ++m) *reinterpret_cast<f32x4*>(&sums[wave][m][i][(lane >> 4) * 4]) = acc[m];
+    __syncthreads();
+    for (int t = threadIdx.x; t < MT * 32; t += NW * 64) {
+        const int p = t >> 1, col = (t & 1) * 8;
+        float v[8] = {};
+        for (int k = 0; k < NW; ++k)
+#pragma unroll
+            for (int j = 0; j < 8; ++j) v[j] += sums[k][p >> 4][p & 15][col + j];
+        if (p < g.P && q0 + col < g.Q) epilogue8<DT>(g, p, q0 + col, v);
+    }
+}
+
+template <int DT, int MT>
+int launch_few_rows(GemmArgs& g, hipStream_t s) {
+    const dim3 grid((unsigned)((g.Q + 15) / 16));
+    // sixteen waves (eight where widening needs the registers) once each has two steps to take, else four
+    constexpr int MANY = DT == F8W ? 8 : 16;
+    const long long bytes = (g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0)) * elem_size(DT);
+    if (bytes >= 32 * 64) hipLaunchKernelGGL((few_rows_kernel<DT, MT, MANY>), grid, dim3(MANY * 64), 0, s, g);
+    else hipLaunchKernelGGL((few_rows_kernel<DT, MT, 4>), grid, dim3(256), 0, s, g);
     NERF_LAUNCH_CHECK();
     return NERF_OK;
 }

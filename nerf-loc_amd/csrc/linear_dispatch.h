@@ -24,18 +24,31 @@ inline bool dma_ok(int layout, const GemmArgs& g) {
 }
 
 template <int DT, int LAY>
-int gemm_fwd(GemmArgs& g, hipStream_t s) {
-    const long long big = ((g.P + 127) / 128) * ((g.Q + 127) / 128) * g.splits;
-    if (big >= 256) return launch<DT, LAY, 128, 128, 2, 2, false>(g, s);
+int gemm_tiles(GemmArgs& g, hipStream_t s) {
+    auto tiles = [&](int n) { return ((g.P + n - 1) / n) * ((g.Q + n - 1) / n) * g.splits; };
+    if (dma_ok<DT>(LAY, g)) {
+        if (LAY == FWD && DT != F8W && tiles(256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, true>(g, s);
+        if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, true>(g, s);
+        return launch<DT, LAY, 64, 64, 2, 2, true>(g, s);
+    }
+    if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, false>(g, s);
     return launch<DT, LAY, 64, 64, 2, 2, false>(g, s);
+}
+
+template <int DT>
+int gemm_forward(GemmArgs& g, hipStream_t s) {
+    if (g.P <= 16) return launch_few_rows<DT == F8 ? F8W : DT, 1>(g, s);
+    if (g.P <= 32) return launch_few_rows<DT == F8 ? F8W : DT, 2>(g, s);
+    if (g.P <= 64) return launch_few_rows<DT == F8 ? F8W : DT, 4>(g, s);
+    return gemm_tiles<DT, FWD>(g, s);
 }
 
 template <int DT>
 int gemm(int layout, GemmArgs& g, hipStream_t s) {
     switch (layout) {
-        case FWD: return gemm_fwd<DT, FWD>(g, s);
-        case DX: return gemm_fwd<DT, DX>(g, s);
-        default: return gemm_fwd<DT, DW>(g, s);
+        case FWD: return gemm_forward<DT>(g, s);
+        case DX: return gemm_tiles<DT, DX>(g, s);
+        default: return gemm_tiles<DT, DW>(g, s);
     }
 }
 

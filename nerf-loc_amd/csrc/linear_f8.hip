@@ -3,6 +3,6 @@
 
 namespace nerf {
 namespace lin {
-int gemm_f8(GemmArgs& g, hipStream_t s) { return gemm_fwd<F8, FWD>(g, s); }
+int gemm_f8(GemmArgs& g, hipStream_t s) { return g.out_dt == F32 ? gemm_forward<F8W>(g, s) : gemm_forward<F8>(g, s); }
 }  // namespace lin
 }  // namespace nerf

@@ -229,19 +229,6 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_grad_kernel(cons
     }
 }
 
-template <int DT>
-__global__ void __launch_bounds__(256) norm_dw_kernel(const float* parts, int n, int N, void* out) {
-    // 64 columns per workgroup, four quarters of the parts side by side
-    __shared__ float quarter[4][64];
-    const int c = blockIdx.x * 64 + (threadIdx.x & 63), q = threadIdx.x >> 6;
-    float s = 0.f;
-    if (c < N)
-        for (int k = q; k < n; k += 4) s += parts[(long long)k * N + c];
-    quarter[q][threadIdx.x & 63] = s;
-    __syncthreads();
-    if (q == 0 && c < N) st_elem(out, c, (quarter[0][threadIdx.x] + quarter[1][threadIdx.x]) + (quarter[2][threadIdx.x] + quarter[3][threadIdx.x]), DT);
-}
-
 constexpr int NORM_MAX = 32768;      // 1024 threads x 4 x 8 columns
 
 // Threads per row: the fewest that hold it in at most four 8-column pieces each.
@@ -287,11 +274,7 @@ static int norm_grad_launch(const NormGradArgs& a, void* dw, hipStream_t s) {
 #undef NERF_CALL
         NERF_LAUNCH_CHECK();
     }
-    if (dw) {
-        hipLaunchKernelGGL(norm_dw_kernel<DT>, dim3((a.N + 63) / 64), dim3(256), 0, s, a.dw_part, (int)blocks, a.N, dw);
-        NERF_LAUNCH_CHECK();
-    }
-    return NERF_OK;
+    return dw ? part_sum(DT, a.dw_part, (int)blocks, 1, a.N, dw, a.N, s) : NERF_OK;
 }
 
 }  // namespace lin

@@ -675,6 +675,23 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 NORM_MAX_WIDTH = 32768
 
 
+def _call(name, dev, *args):
+    """lib().name(*args, current stream) with dev current.  Tensors' pointers travel as plain integers, and the device is
+    switched only where it has to be: at the smallest sizes the call costs more than the kernel."""
+    fn = getattr(lib(), name)
+    if torch.cuda.current_device() == dev.index:
+        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    else:
+        with torch.cuda.device(dev):
+            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+    if code != 0:
+        _check(code, name)
+
+
+def _at(t):
+    return None if t is None else t.data_ptr()
+
+
 def activation_code(name):
     if name not in ACTIVATIONS:
         raise ValueError("unknown activation %r (one of %s)" % (name, ", ".join(repr(k) for k in ACTIVATIONS)))
@@ -737,9 +754,8 @@ def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)
     y = torch.empty((M, N), dtype=dt, device=dev)
     z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
-    with torch.cuda.device(dev):
-        _check(lib().nerf_linear(DTYPES[dt], _ptr(x0), ld0, k0, _ptr(x1), ld1, k1, _ptr(w), ldw, _ptr(b), act, _ptr(r), ldr,
-                                 _ptr(y), N, _ptr(z), N, M, N, _stream(y)), "nerf_linear")
+    _call("nerf_linear", dev, DTYPES[dt], _at(x0), ld0, k0, _at(x1), ld1, k1, _at(w), ldw, _at(b), act, _at(r), ldr,
+                                 _at(y), N, _at(z), N, M, N)
     return y, z
 
 
@@ -759,10 +775,9 @@ def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=Tru
     db = new(N) if want_b else None
     nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], M, N, k0, k1, act)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)      # its own in every call: calls on other streams may overlap
-    with torch.cuda.device(dev):
-        _check(lib().nerf_linear_backward(DTYPES[dt], _ptr(g), ldg, _ptr(zz), ldz, act, _ptr(x0), ld0, k0, _ptr(x1), ld1, k1,
-                                          _ptr(w), ldw, _ptr(dx0), k0, _ptr(dx1), k1, _ptr(dw), _ptr(db), M, N, _ptr(ws),
-                                          nbytes, _stream(g)), "nerf_linear_backward")
+    _call("nerf_linear_backward", dev, DTYPES[dt], _at(g), ldg, _at(zz), ldz, act, _at(x0), ld0, k0, _at(x1), ld1, k1,
+                                          _at(w), ldw, _at(dx0), k0, _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws),
+                                          nbytes)
     return dx0, dx1, dw, db
 
 
@@ -786,9 +801,8 @@ def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=Non
     b = None if bias is None else _vector(bias, "bias", N, out_dtype, dev)
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_dtype, dev)
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    with torch.cuda.device(dev):
-        _check(lib().nerf_linear_q8(_ptr(xq), ldx, _ptr(xs), _ptr(wq), ldw, _ptr(ws), DTYPES[out_dtype], _ptr(b), act, _ptr(r),
-                                    ldr, _ptr(y), N, M, N, K, _stream(y)), "nerf_linear_q8")
+    _call("nerf_linear_q8", dev, _at(xq), ldx, _at(xs), _at(wq), ldw, _at(ws), DTYPES[out_dtype], _at(b), act, _at(r),
+                                    ldr, _at(y), N, M, N, K)
     return y
 
 
@@ -813,9 +827,8 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6, want_h=True, want_rstd=Fals
     q = torch.empty((M, N), dtype=torch.float8_e4m3fn, device=dev) if q8 else None
     scale = torch.empty((M,), dtype=torch.float32, device=dev) if q8 else None
     rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
-    with torch.cuda.device(dev):
-        _check(lib().nerf_add_rms_norm(DTYPES[dt], _ptr(x), ldx, _ptr(r), ldr, _ptr(w), float(eps), _ptr(h), N, _ptr(y), N,
-                                       _ptr(q), N, _ptr(scale), _ptr(rstd), M, N, _stream(x)), "nerf_add_rms_norm")
+    _call("nerf_add_rms_norm", dev, DTYPES[dt], _at(x), ldx, _at(r), ldr, _at(w), float(eps), _at(h), N, _at(y), N,
+                                       _at(q), N, _at(scale), _at(rstd), M, N)
     return (q, scale, h) if q8 else (y, h, rstd)
 
 
@@ -832,8 +845,6 @@ def add_rms_norm_backward(gy, h, weight, rstd, gh=None, want_x=True, want_w=True
         return None, None
     nbytes = lib().nerf_add_rms_norm_backward_workspace_bytes(M, N) if want_w else 0
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
-    with torch.cuda.device(dev):
-        _check(lib().nerf_add_rms_norm_backward(DTYPES[dt], _ptr(gy), ldgy, _ptr(gh), ldgh, _ptr(h), ldh, _ptr(w), _ptr(rstd),
-                                                _ptr(dx), N, _ptr(dw), M, N, _ptr(ws), nbytes, _stream(h)),
-               "nerf_add_rms_norm_backward")
+    _call("nerf_add_rms_norm_backward", dev, DTYPES[dt], _at(gy), ldgy, _at(gh), ldgh, _at(h), ldh, _at(w), _at(rstd),
+                                                _at(dx), N, _at(dw), M, N, _at(ws), nbytes)
     return dx, dw

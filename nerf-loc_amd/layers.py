@@ -71,8 +71,11 @@ def linear(x, weight, bias=None, activation=None, residual=None):
         r = _flat(residual, "residual")
         if tuple(residual.shape[:-1]) != lead:
             raise ValueError("residual has leading shape %s, x %s" % (tuple(residual.shape[:-1]), lead))
-    y = _LinearFn.apply(a, b, weight, bias, r, "none" if activation is None else activation)
-    return y if len(lead) == 1 else y.reshape(lead + (y.shape[-1],))
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (a, b, weight, bias, r)):
+        y = _LinearFn.apply(a, b, weight, bias, r, "none" if activation is None else activation)
+    else:
+        y, _ = hip.linear(a, weight, bias, activation, r, b)
+    return y if len(lead) == 1 else y.reshape(lead + y.shape[-1:])
 
 
 class _AddNormFn(torch.autograd.Function):
@@ -108,13 +111,18 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
 
     In 16-bit types y comes from the float32 sum, h is that sum rounded, and the backward starts from the rounded h."""
     a = _flat(x, "x")
-    if residual is None:
-        y = _AddNormFn.apply(a, weight, None, float(eps))
-        return y.reshape(x.shape), x
-    if tuple(residual.shape) != tuple(x.shape):
-        raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
-    y, h = _AddNormFn.apply(a, weight, _flat(residual, "residual"), float(eps))
-    return y.reshape(x.shape), h.reshape(x.shape)
+    r = None
+    if residual is not None:
+        if residual.shape != x.shape:
+            raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
+        r = _flat(residual, "residual")
+    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (a, weight, r)):
+        out = _AddNormFn.apply(a, weight, r, float(eps))
+        y, h = out if r is not None else (out, x)
+    else:
+        y, h, _ = hip.add_rms_norm(a, weight, r, eps, want_h=r is not None)
+        h = x if h is None else h
+    return (y, h) if x.dim() == 2 else (y.reshape(x.shape), h.reshape(x.shape))
 
 
 def _no_grad(what, *tensors):

@@ -460,3 +460,99 @@ def test_add_rms_norm_q8(dev, dtype, size):
 # ---------------------------------------------------------------------------------------------------- 8-bit linear
 Q8_SIZES = [(1, 1, 1), (1, 4096, 1024), (3, 50, 16), (5, 256, 300), (17, 63, 129), (64, 128, 128), (130, 257, 511), (300, 512, 1024),
             (1024, 640, 256), (513, 33, 48)]
+
+
+def q8_operands(dev, m, n, k, seed):
+    g = torch.Generator(device=dev).manual_seed(seed)
+
+    def rows(r, c, scale):
+        x = torch.randn(r, c, device=dev, generator=g) * scale
+        s = (x.abs().amax(-1) / 448).clamp_min(2.0 ** -126)
+        return (x / s[:, None]).to(torch.float8_e4m3fn), s
+    return rows(m, k, 1.0) + rows(n, k, k ** -0.5) + (g,)
+
+
+def group_cut(x, w):
+    """What the 8-bit matrix instruction may cut off: of every aligned group of eight products each loses less than 2^-13
+    of the largest."""
+    m, k = x.shape
+    pad = -k % 8
+    x, w = torch.nn.functional.pad(x, (0, pad)), torch.nn.functional.pad(w, (0, pad))
+    cut = torch.zeros(m, w.shape[0], dtype=torch.float64, device=x.device)
+    for i in range(0, k + pad, 8):
+        cut += (x[:, None, i:i + 8] * w[None, :, i:i + 8]).abs().amax(-1)
+    return cut * (7 * 2.0 ** -13)
+
+
+@pytest.mark.parametrize("size", Q8_SIZES, ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_q8(dev, dtype, size):
+    m, n, k = size
+    dt = TYPES[dtype]
+    i = Q8_SIZES.index(size)
+    act = ACTS[i % 4]
+    xq, xs, wq, ws, g = q8_operands(dev, m, n, k, 400 + i)
+    b = (torch.randn(n, device=dev, generator=g) * 0.1).to(dt) if i % 3 else None
+    r = torch.randn(m, n, device=dev, generator=g).to(dt) if i % 2 else None
+    y = layers.linear_q8(xq, xs, wq, ws, b, act, r, out_dtype=dt)
+    assert y.dtype == dt
+    X, W, S, T = xq.double(), wq.double(), xs.double()[:, None], ws.double()
+    z = X @ W.t().contiguous() * S * T
+    ez = (k + 6) * E * (X.abs() @ W.abs().t().contiguous()) * S * T
+    if dt != torch.float32:
+        ez = ez + group_cut(X, W) * S * T
+    if b is not None:
+        z = z + b.double()
+        ez = ez + E * z.abs()
+    want = act64(z, act)
+    err = SLOPE * ez + (0 if act in ("none", "relu") else ACT_ERR * (1 + z.abs()))
+    if r is not None:
+        want = want + r.double()
+        err = err + E * want.abs()
+    check(y, want, err + half_step(dt) * (want.abs() + err) + tiny(dt), "y")
+
+
+def test_linear_q8_views_every_number_and_no_rows(dev):
+    """All 254 finite e4m3 numbers, exactly; strided operands; NaN; an empty batch; leading dimensions."""
+    codes = torch.tensor([c for c in range(256) if c & 127 != 127], dtype=torch.uint8, device=dev)
+    v = codes.view(torch.float8_e4m3fn)
+    eye = torch.eye(254, device=dev).to(torch.float8_e4m3fn)
+    one = torch.ones(254, device=dev)
+    x = torch.diag(v.float()).to(torch.float8_e4m3fn)
+    for dt in TYPES.values():
+        y = layers.linear_q8(x, one, eye, one, out_dtype=dt)
+        assert torch.equal(y.float(), torch.diag(v.float()))
+    xq, xs, wq, ws, g = q8_operands(dev, 96, 40, 77, 9)
+    big = torch.zeros(96, 131, device=dev, dtype=torch.float8_e4m3fn).view(torch.uint8).fill_(0x7f).view(torch.float8_e4m3fn)
+    big.view(torch.uint8)[:, 5:82] = xq.view(torch.uint8)
+    want = layers.linear_q8(xq, xs, wq, ws, activation="silu")
+    assert torch.equal(layers.linear_q8(big[:, 5:82], xs, wq, ws, activation="silu"), want)
+    assert torch.equal(layers.linear_q8(xq.reshape(4, 24, 77), xs.reshape(4, 24), wq, ws, activation="silu"), want.reshape(4, 24, 40))
+    bad = xq.clone()
+    bad.view(torch.uint8)[95, 76] = 0x7f
+    y = layers.linear_q8(bad, xs, wq, ws, activation="silu")
+    assert bool(torch.isnan(y[95]).all()) and torch.equal(y[:95], want[:95])
+    assert tuple(layers.linear_q8(xq[:0], xs[:0], wq, ws).shape) == (0, 40)
+
+
+def test_quantised_block_as_it_is_used(dev):
+    """Norm to 8 bits, 8-bit layer with the residual, next norm: against the same block on the quantised numbers in 64
+    bits, and near the unquantised one."""
+    g = torch.Generator(device=dev).manual_seed(11)
+    x, r = (torch.randn(200, 320, device=dev, generator=g).bfloat16() for _ in range(2))
+    w = (torch.randn(320, 320, device=dev, generator=g) * 320 ** -0.5)
+    wn = torch.ones(320, device=dev, dtype=torch.bfloat16)
+    wq, ws = layers.quantize_weight(w)
+    q, s, h = layers.add_rms_norm_q8(x, wn, r)
+    y = layers.linear_q8(q, s, wq, ws, activation="relu", residual=h)
+    n2, h2 = layers.add_rms_norm(y, wn, h)
+    X, W = q.double() * s.double()[:, None], wq.double() * ws.double()[:, None]
+    z = X @ W.t().contiguous()
+    ey = (330 * E) * (X.abs() @ W.abs().t().contiguous()) + group_cut(q.double(), wq.double()) * s.double()[:, None] * ws.double()
+    want = torch.relu(z) + h.double()
+    check(y, want, ey + half_step(torch.bfloat16) * (want.abs() + ey), "block")
+    hh, _, nn = norm64(y, wn, h, 1e-6)
+    check(n2, nn, nn.abs() * (175 * E + half_step(torch.bfloat16)) + 1e-30, "norm")
+    full = torch.relu((norm64(x, wn, r, 1e-6)[2]) @ w.double().t().contiguous()) + h.double()
+    # each factor is off by at most 2^-4 of itself, in effect independently: 2^-4 / sqrt 3 each, together below 2^-4
+    assert float((y.double() - full).norm() / (full - h.double()).norm()) < 2.0 ** -4
