@@ -675,15 +675,20 @@ ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 NORM_MAX_WIDTH = 32768
 
 
+_CALLS = {}
+
+
 def _call(name, dev, *args):
     """lib().name(*args, current stream) with dev current.  Tensors' pointers travel as plain integers, and the device is
     switched only where it has to be: at the smallest sizes the call costs more than the kernel."""
-    fn = getattr(lib(), name)
+    fn = _CALLS.get(name)
+    if fn is None:
+        fn = _CALLS[name] = getattr(lib(), name)
     if torch.cuda.current_device() == dev.index:
-        code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+        code = fn(*args, torch.cuda.current_stream().cuda_stream)
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, torch.cuda.current_stream(dev).cuda_stream)
+            code = fn(*args, torch.cuda.current_stream().cuda_stream)
     if code != 0:
         _check(code, name)
 
@@ -698,28 +703,39 @@ def activation_code(name):
     return ACTIVATIONS[name]
 
 
-def _matrix(t, name, rows=None, cols=None, dtype=None, device=None):
-    """A [rows, cols] device matrix as the layer kernels take it: columns contiguous, any row stride of at least its row's
-    length.  Other layouts (transposed, expanded rows) are copied.  Returns (tensor, row stride)."""
+def _matrix_error(t, name, rows, cols, dtype, device):
+    """Why t is not the [rows, cols] matrix that is wanted (None: any)."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
     if not t.is_cuda:
         raise ValueError("%s must live on a GPU (got %s); this engine has no CPU path" % (name, t.device))
     if device is not None and t.device != device:
         raise ValueError("%s is on %s but %s was expected" % (name, t.device, device))
-    if t.dtype != dtype and dtype is not None:
-        raise ValueError("%s must be %s like the input, got %s" % (name, dtype, t.dtype))
-    if t.dim() != 2 or (rows is not None and t.shape[0] != rows) or (cols is not None and t.shape[1] != cols):
-        raise ValueError("%s must be [%s, %s], got %s" % (name, "n" if rows is None else rows, "n" if cols is None else cols, tuple(t.shape)))
-    if (t.shape[1] > 1 and t.stride(1) != 1) or (t.shape[0] > 1 and t.stride(0) < t.shape[1]):
+    if dtype is not None and t.dtype != dtype:
+        raise ValueError("%s must be %s, got %s" % (name, dtype, t.dtype))
+    raise ValueError("%s must be [%s, %s], got %s" % (name, "n" if rows is None else rows, "n" if cols is None else cols, tuple(t.shape)))
+
+
+def _matrix(t, name, rows=None, cols=None, dtype=None, device=None):
+    """A [rows, cols] device matrix as the layer kernels take it: columns contiguous, any row stride of at least its row's
+    length.  Other layouts (transposed, expanded rows) are copied.  Returns (tensor, row stride, rows, columns)."""
+    if not isinstance(t, torch.Tensor) or not t.is_cuda or t.dim() != 2:
+        _matrix_error(t, name, rows, cols, dtype, device)
+    m, n = t.shape
+    if (device is not None and t.device != device) or (dtype is not None and t.dtype is not dtype) or \
+            (rows is not None and m != rows) or (cols is not None and n != cols):
+        _matrix_error(t, name, rows, cols, dtype, device)
+    s0, s1 = t.stride()
+    if (n > 1 and s1 != 1) or (m > 1 and s0 < n):
         t = t.contiguous()
-    return t, max(t.stride(0), t.shape[1])
+        s0 = n
+    return t, (s0 if s0 > n else n), m, n
 
 
 def _vector(t, name, n, dtype, device):
     if not isinstance(t, torch.Tensor):
         raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
-    if not t.is_cuda or t.device != device or t.dtype != dtype or tuple(t.shape) != (n,):
+    if t.dtype is not dtype or t.device != device or t.dim() != 1 or t.shape[0] != n:
         raise ValueError("%s must be %s [%d] on %s, got %s %s on %s" % (name, dtype, n, device, t.dtype, tuple(t.shape), t.device))
     return t if t.is_contiguous() else t.contiguous()
 
@@ -731,31 +747,32 @@ def _layer_dtype(t, name):
 
 def _layer_input(x0, x1, weight):
     _layer_dtype(x0, "x")
-    x0, ld0 = _matrix(x0, "x")
-    M, k0 = x0.shape
+    x0, ld0, M, k0 = _matrix(x0, "x")
+    dt, dev = x0.dtype, x0.device
     ld1, k1 = 0, 0
     if x1 is not None:
-        x1, ld1 = _matrix(x1, "the second piece of x", rows=M, dtype=x0.dtype, device=x0.device)
-        k1 = x1.shape[1]
-        _need(k1 >= 1, "the second piece of x has no columns")
-    _need(k0 >= 1, "x has no columns")
-    w, ldw = _matrix(weight, "weight", cols=k0 + k1, dtype=x0.dtype, device=x0.device)
-    _need(w.shape[0] >= 1, "weight has no rows")
-    return x0, ld0, k0, x1, ld1, k1, w, ldw
+        x1, ld1, _, k1 = _matrix(x1, "the second piece of x", M, None, dt, dev)
+        if k1 < 1:
+            raise ValueError("the second piece of x has no columns")
+    if k0 < 1:
+        raise ValueError("x has no columns")
+    w, ldw, N, _ = _matrix(weight, "weight", None, k0 + k1, dt, dev)
+    if N < 1:
+        raise ValueError("weight has no rows")
+    return x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev
 
 
 def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_z=False):
     """act([x0 | x1] weight^T + bias) + residual on matrices [M, k0], [M, k1], [N, k0 + k1], [N], [M, N] of one type.
     Returns (y, z): z is the argument of act with want_z, else None."""
     act = activation_code(activation)
-    x0, ld0, k0, x1, ld1, k1, w, ldw = _layer_input(x0, x1, weight)
-    M, N, dt, dev = x0.shape[0], w.shape[0], x0.dtype, x0.device
+    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = _layer_input(x0, x1, weight)
     b = None if bias is None else _vector(bias, "bias", N, dt, dev)
-    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)[:2]
     y = torch.empty((M, N), dtype=dt, device=dev)
     z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
     _call("nerf_linear", dev, DTYPES[dt], _at(x0), ld0, k0, _at(x1), ld1, k1, _at(w), ldw, _at(b), act, _at(r), ldr,
-                                 _at(y), N, _at(z), N, M, N)
+          _at(y), N, _at(z), N, M, N)
     return y, z
 
 
@@ -763,11 +780,10 @@ def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=Tru
     """Gradients of linear for g = dL/dy: (dx0, dx1, dweight, dbias), None where not wanted.  z: the argument of act that
     the forward gave (for relu without a residual, y)."""
     act = activation_code(activation)
-    x0, ld0, k0, x1, ld1, k1, w, ldw = _layer_input(x0, x1, weight)
-    M, N, dt, dev = x0.shape[0], w.shape[0], x0.dtype, x0.device
-    g, ldg = _matrix(g, "the gradient of y", M, N, dt, dev)
+    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = _layer_input(x0, x1, weight)
+    g, ldg, _, _ = _matrix(g, "the gradient of y", M, N, dt, dev)
     _need(act == 0 or z is not None, "linear_backward: the gradient through %s needs z", activation)
-    zz, ldz = (None, 0) if act == 0 else _matrix(z, "z", M, N, dt, dev)
+    zz, ldz = (None, 0) if act == 0 else _matrix(z, "z", M, N, dt, dev)[:2]
     new = lambda *shape: torch.empty(shape, dtype=dt, device=dev)
     dx0 = new(M, k0) if want_x0 else None
     dx1 = new(M, k1) if want_x1 and x1 is not None else None
@@ -776,7 +792,7 @@ def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=Tru
     nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], M, N, k0, k1, act)
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)      # its own in every call: calls on other streams may overlap
     _call("nerf_linear_backward", dev, DTYPES[dt], _at(g), ldg, _at(zz), ldz, act, _at(x0), ld0, k0, _at(x1), ld1, k1,
-                                          _at(w), ldw, _at(dx0), k0, _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws),
+          _at(w), ldw, _at(dx0), k0, _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws),
                                           nbytes)
     return dx0, dx1, dw, db
 
@@ -789,30 +805,29 @@ def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=Non
     f8 = torch.float8_e4m3fn
     _need(isinstance(xq, torch.Tensor) and xq.dtype == f8, "xq must be float8_e4m3fn, got %s",
           xq.dtype if isinstance(xq, torch.Tensor) else type(xq).__name__)
-    xq, ldx = _matrix(xq, "xq")
-    M, K = xq.shape
+    xq, ldx, M, K = _matrix(xq, "xq")
     dev = xq.device
     _need(K >= 1, "xq has no columns")
-    wq, ldw = _matrix(wq, "wq", cols=K, dtype=f8, device=dev)
-    N = wq.shape[0]
+    wq, ldw, N, _ = _matrix(wq, "wq", None, K, f8, dev)
     _need(N >= 1, "wq has no rows")
     xs = _vector(x_scale, "x_scale", M, torch.float32, dev)
     ws = _vector(w_scale, "w_scale", N, torch.float32, dev)
     b = None if bias is None else _vector(bias, "bias", N, out_dtype, dev)
-    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_dtype, dev)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_dtype, dev)[:2]
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
     _call("nerf_linear_q8", dev, _at(xq), ldx, _at(xs), _at(wq), ldw, _at(ws), DTYPES[out_dtype], _at(b), act, _at(r),
-                                    ldr, _at(y), N, M, N, K)
+          ldr, _at(y), N, M, N, K)
     return y
 
 
 def _norm_input(x, weight, residual):
     _layer_dtype(x, "x")
-    x, ldx = _matrix(x, "x")
-    M, N = x.shape
-    _need(1 <= N <= NORM_MAX_WIDTH, "add_rms_norm: rows of 1 to %d columns, got %d", NORM_MAX_WIDTH, N)
-    w = _vector(weight, "weight", N, x.dtype, x.device)
-    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, x.dtype, x.device)
+    x, ldx, M, N = _matrix(x, "x")
+    dt, dev = x.dtype, x.device
+    if not 1 <= N <= NORM_MAX_WIDTH:
+        raise ValueError("add_rms_norm: rows of 1 to %d columns, got %d" % (NORM_MAX_WIDTH, N))
+    w = _vector(weight, "weight", N, dt, dev)
+    r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)[:2]
     return x, ldx, M, N, w, r, ldr
 
 
@@ -828,7 +843,7 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6, want_h=True, want_rstd=Fals
     scale = torch.empty((M,), dtype=torch.float32, device=dev) if q8 else None
     rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
     _call("nerf_add_rms_norm", dev, DTYPES[dt], _at(x), ldx, _at(r), ldr, _at(w), float(eps), _at(h), N, _at(y), N,
-                                       _at(q), N, _at(scale), _at(rstd), M, N)
+          _at(q), N, _at(scale), _at(rstd), M, N)
     return (q, scale, h) if q8 else (y, h, rstd)
 
 
@@ -836,8 +851,8 @@ def add_rms_norm_backward(gy, h, weight, rstd, gh=None, want_x=True, want_w=True
     """(dx, dweight) of add_rms_norm for gy = dL/dy and gh = dL/dh; dx is the residual's gradient too."""
     h, ldh, M, N, w, _, _ = _norm_input(h, weight, None)
     dt, dev = h.dtype, h.device
-    gy, ldgy = _matrix(gy, "the gradient of y", M, N, dt, dev)
-    gh, ldgh = (None, 0) if gh is None else _matrix(gh, "the gradient of h", M, N, dt, dev)
+    gy, ldgy, _, _ = _matrix(gy, "the gradient of y", M, N, dt, dev)
+    gh, ldgh = (None, 0) if gh is None else _matrix(gh, "the gradient of h", M, N, dt, dev)[:2]
     rstd = _vector(rstd, "rstd", M, torch.float32, dev)
     dx = torch.empty((M, N), dtype=dt, device=dev) if want_x else None
     dw = torch.empty((N,), dtype=dt, device=dev) if want_w else None
@@ -846,5 +861,5 @@ def add_rms_norm_backward(gy, h, weight, rstd, gh=None, want_x=True, want_w=True
     nbytes = lib().nerf_add_rms_norm_backward_workspace_bytes(M, N) if want_w else 0
     ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)
     _call("nerf_add_rms_norm_backward", dev, DTYPES[dt], _at(gy), ldgy, _at(gh), ldgh, _at(h), ldh, _at(w), _at(rstd),
-                                                _at(dx), N, _at(dw), M, N, _at(ws), nbytes)
+          _at(dx), N, _at(dw), M, N, _at(ws), nbytes)
     return dx, dw

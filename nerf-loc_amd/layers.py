@@ -18,6 +18,20 @@ from torch.autograd.function import once_differentiable
 from . import hip
 
 
+def _wants_grad(*tensors):
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _tensors(**named):
+    for name, t in named.items():
+        if t is not None and not isinstance(t, torch.Tensor):
+            raise TypeError("%s must be a torch.Tensor, got %s" % (name, type(t).__name__))
+
+
 def _flat(t, name):
     """[..., n] -> [m, n] without a copy where the layout allows it."""
     if not isinstance(t, torch.Tensor):
@@ -60,22 +74,22 @@ def linear(x, weight, bias=None, activation=None, residual=None):
     bias [N]; residual [..., N] (exactly the result's shape); activation None, "relu", "gelu" (the exact one) or "silu"."""
     x0, x1 = x if isinstance(x, (tuple, list)) and len(x) == 2 else (x, None)
     a = _flat(x0, "x")
-    lead = tuple(x0.shape[:-1])
-    b = None
+    lead = None if a is x0 else x0.shape[:-1]          # None: matrices all along
+    b = r = None
     if x1 is not None:
         b = _flat(x1, "the second piece of x")
-        if tuple(x1.shape[:-1]) != lead:
-            raise ValueError("the pieces of x have leading shapes %s and %s" % (lead, tuple(x1.shape[:-1])))
-    r = None
+        if x1.shape[:-1] != x0.shape[:-1]:
+            raise ValueError("the pieces of x have leading shapes %s and %s" % (tuple(x0.shape[:-1]), tuple(x1.shape[:-1])))
     if residual is not None:
         r = _flat(residual, "residual")
-        if tuple(residual.shape[:-1]) != lead:
-            raise ValueError("residual has leading shape %s, x %s" % (tuple(residual.shape[:-1]), lead))
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (a, b, weight, bias, r)):
+        if residual.shape[:-1] != x0.shape[:-1]:
+            raise ValueError("residual has leading shape %s, x %s" % (tuple(residual.shape[:-1]), tuple(x0.shape[:-1])))
+    _tensors(weight=weight, bias=bias)
+    if _wants_grad(a, b, weight, bias, r):
         y = _LinearFn.apply(a, b, weight, bias, r, "none" if activation is None else activation)
     else:
         y, _ = hip.linear(a, weight, bias, activation, r, b)
-    return y if len(lead) == 1 else y.reshape(lead + y.shape[-1:])
+    return y if lead is None else y.reshape(lead + y.shape[-1:])
 
 
 class _AddNormFn(torch.autograd.Function):
@@ -116,7 +130,8 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
         if residual.shape != x.shape:
             raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
         r = _flat(residual, "residual")
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in (a, weight, r)):
+    _tensors(weight=weight)
+    if _wants_grad(a, weight, r):
         out = _AddNormFn.apply(a, weight, r, float(eps))
         y, h = out if r is not None else (out, x)
     else:
@@ -126,37 +141,41 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
 
 
 def _no_grad(what, *tensors):
-    if torch.is_grad_enabled() and any(isinstance(t, torch.Tensor) and t.requires_grad for t in tensors):
+    if _wants_grad(*tensors):
         raise NotImplementedError("%s has no gradient (8-bit numbers are for inference): call it under torch.no_grad()" % what)
 
 
 def add_rms_norm_q8(x, weight, residual=None, eps=1e-6):
     """add_rms_norm with y in 8 bits: returns (q, scale, h), q float8_e4m3fn like x and scale float32 [...], y = scale q.
     scale = max(max|y| / 448, 2^-126) of its row; a row with an infinity or NaN reads back as NaN."""
+    _tensors(x=x, weight=weight, residual=residual)
     _no_grad("add_rms_norm_q8", x, weight, residual)
     a = _flat(x, "x")
     r = None
     if residual is not None:
-        if tuple(residual.shape) != tuple(x.shape):
+        if residual.shape != x.shape:
             raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
         r = _flat(residual, "residual")
     q, scale, h = hip.add_rms_norm(a, weight, r, eps, want_h=r is not None, q8=True)
-    return q.reshape(x.shape), scale.reshape(x.shape[:-1]), x if h is None else h.reshape(x.shape)
+    if h is None:
+        h = a
+    return (q, scale, h) if a is x else (q.reshape(x.shape), scale.reshape(x.shape[:-1]), h.reshape(x.shape))
 
 
 def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
     """act(x W^T + bias) + residual with x = x_scale xq (xq float8_e4m3fn [..., K], x_scale float32 [...]) and
     W = w_scale wq ([N, K], [N]); bias, residual and the result are of out_dtype.  No gradient."""
+    _tensors(xq=xq, x_scale=x_scale, wq=wq, w_scale=w_scale, bias=bias, residual=residual)
     _no_grad("linear_q8", x_scale, w_scale, bias, residual)
     a = _flat(xq, "xq")
-    lead = tuple(xq.shape[:-1])
-    if not isinstance(x_scale, torch.Tensor) or tuple(x_scale.shape) != lead:
-        raise ValueError("x_scale must be a tensor of shape %s" % (lead,))
-    if residual is not None and tuple(residual.shape[:-1]) != lead:
-        raise ValueError("residual has leading shape %s, xq %s" % (tuple(residual.shape[:-1]), lead))
-    y = hip.linear_q8(a, x_scale.reshape(-1), wq, w_scale, bias, activation,
+    lead = xq.shape[:-1]
+    if x_scale.shape != lead:
+        raise ValueError("x_scale must be of shape %s, got %s" % (tuple(lead), tuple(x_scale.shape)))
+    if residual is not None and residual.shape[:-1] != lead:
+        raise ValueError("residual has leading shape %s, xq %s" % (tuple(residual.shape[:-1]), tuple(lead)))
+    y = hip.linear_q8(a, x_scale if a is xq else x_scale.reshape(-1), wq, w_scale, bias, activation,
                       None if residual is None else _flat(residual, "residual"), out_dtype)
-    return y if len(lead) == 1 else y.reshape(lead + (y.shape[-1],))
+    return y if a is xq else y.reshape(lead + y.shape[-1:])
 
 
 @torch.no_grad()
