@@ -364,52 +364,105 @@ __device__ __forceinline__ uint4 part_chunk(const char* p, int have) {
     return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
 }
 
-// One operand's side of the main loop.  A tile's chunks lie at fixed offsets from its first element, worked out once per
-// piece of the reduction; only a k-tile that runs over the reduction's end looks at every chunk again.
-template <int DT, int TR, int OUT, int NT, bool DMA>
+// The 16 bytes at v moved down by n (0 .. 15), zeros from above.
+__device__ __forceinline__ uint4 move_down(const uint4& v, int n) {
+    unsigned long long lo = (unsigned long long)v.y << 32 | v.x, hi = (unsigned long long)v.w << 32 | v.z;
+    const int b = 8 * (n & 7);
+    if (n >= 8) { lo = hi; hi = 0; }
+    if (b) {
+        lo = lo >> b | hi << (64 - b);
+        hi >>= b;
+    }
+    return make_uint4((unsigned)lo, (unsigned)(lo >> 32), (unsigned)hi, (unsigned)(hi >> 32));
+}
+
+// How an operand's tile reaches LDS.
+//   DMA16  by LDS-DMA in 16-byte chunks: rows on 16 bytes, whole chunks throughout
+//   REGS   through registers, any alignment (16-byte global loads take it).  Word-wise LDS-DMA of unaligned float32 rows
+//          was no faster (4096^3 with rows of 4095: 1359 us against 1314): each row's lines are fetched twice either way
+enum Way { REGS = 0, DMA16 = 1 };
+
+// One operand's side of the main loop.  A tile's pieces lie at fixed offsets from its first element, worked out once per
+// piece of the reduction; only a k-tile that runs over the reduction's end looks at them again.
+template <int DT, int TR, int OUT, int NT, int WAY>
 struct Loader {
     using T = Tile<DT, TR, OUT, NT>;
-    uint4 st[DMA ? 1 : T::CH];
-    unsigned off[T::CH];         // bytes from the tile's first element
-    bool fast;                   // whole k-tiles need no check: rows are there (or doubled), chunks of outputs are whole
+    static constexpr int N = T::CH;          // chunks per thread
+    uint4 st[WAY == REGS ? T::CH : 1];
+    unsigned off[N];             // bytes from the tile's first element
+    int down[WAY == REGS && TR ? T::CH : 1];
+    bool fast, edge;
+
+    __device__ __forceinline__ static int row_of(int i, int tid) { return T::row_of(i * NT + tid); }
+    __device__ __forceinline__ static int col_of(int i, int tid) { return T::col_of(i * NT + tid); }
 
     // outs: rows of C this operand has from the tile's first on
     __device__ __forceinline__ void start(long long ld, long long outs, int tid) {
         const int no = (int)(outs < OUT ? outs : OUT);
-        fast = DMA || ((!TR || no == OUT) && ld * T::E * 256 < (1ll << 31));
+        if constexpr (WAY != REGS) {
+            // what lies behind the last row of C reads as zeros
 #pragma unroll
-        for (int i = 0; i < T::CH; ++i) {
-            const int L = i * NT + tid;
-            const int row = T::row_of(L), col = T::col_of(L);
-            // rows behind the last: zeros by LDS-DMA; the last one again by loads (what they give is never stored)
-            if constexpr (DMA) off[i] = (TR ? col : row) < no ? (unsigned)(row * (int)ld + col) * T::E : OUTSIDE;
-            else off[i] = fast ? (unsigned)((TR || row < no ? row : no - 1) * (int)ld + col) * T::E : 0u;
+            for (int i = 0; i < N; ++i) {
+                const int row = row_of(i, tid), col = col_of(i, tid);
+                off[i] = (TR ? col : row) < no ? (unsigned)(row * (int)ld + col) * T::E : OUTSIDE;
+            }
+        } else {
+            // what lies behind the last row of C repeats it or is anything: it is never stored.  A chunk that runs over a
+            // reduction-major row's end is read from its last 16 bytes instead and moved down.
+            fast = ld * T::E * 256 < (1ll << 31) && (!TR || no >= T::CE);
+            edge = TR && no < OUT;
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                int row = row_of(i, tid), col = col_of(i, tid);
+                if (!TR && row >= no) row = no - 1;
+                if constexpr (TR) {
+                    const int c = col + T::CE <= no ? col : no - T::CE;
+                    down[i] = col < no ? (col - c) * T::E : 0;
+                    col = c;
+                }
+                off[i] = fast ? (unsigned)(row * (int)ld + col) * T::E : 0u;
+            }
         }
     }
-    // base: the tile's first element at this k-tile; reds: what is left of the reduction from there
-    __device__ __forceinline__ void fetch(const char* base, long long ld, long long outs, long long reds, int tid, unsigned lds) {
-        if constexpr (DMA) {
+    // base: the tile's first element at this k-tile; done / reds: the reduction in front of it and what is left from there
+    __device__ __forceinline__ void fetch(const char* base, long long ld, long long outs, long long done, long long reds, int tid, unsigned lds) {
+        if constexpr (WAY != REGS) {
             const i32x4 rsrc = buffer_of(base);
             const unsigned at = lds + __builtin_amdgcn_readfirstlane(tid >> 6) * 1024;
             if (reds >= T::BK) {
 #pragma unroll
-                for (int i = 0; i < T::CH; ++i) dma16(at + i * NT * 16, off[i], rsrc);
+                for (int i = 0; i < N; ++i) dma16(at + i * NT * 16, off[i], rsrc);
             } else {
 #pragma unroll
-                for (int i = 0; i < T::CH; ++i) {
-                    const int L = i * NT + tid;
-                    dma16(at + i * NT * 16, (TR ? T::row_of(L) : T::col_of(L)) < reds ? off[i] : OUTSIDE, rsrc);
-                }
+                for (int i = 0; i < N; ++i)
+                    dma16(at + i * NT * 16, (TR ? row_of(i, tid) : col_of(i, tid)) < reds ? off[i] : OUTSIDE, rsrc);
             }
         } else if (fast && reds >= T::BK) {
 #pragma unroll
-            for (int i = 0; i < T::CH; ++i) __builtin_memcpy(&st[i], base + off[i], 16);      // any alignment: global loads take it
+            for (int i = 0; i < N; ++i) __builtin_memcpy(&st[i], base + off[i], 16);
+            if constexpr (TR) {
+                if (edge) {
+#pragma unroll
+                    for (int i = 0; i < N; ++i) st[i] = move_down(st[i], down[i]);
+                }
+            }
+        } else if (fast && (TR || done + reds >= T::CE)) {
+            // the reduction's last k-tile: zeros behind its end
+#pragma unroll
+            for (int i = 0; i < N; ++i) {
+                const int at = TR ? row_of(i, tid) : col_of(i, tid), nr = (int)reds;
+                st[i] = make_uint4(0, 0, 0, 0);
+                if (at < nr) {
+                    const int back = TR || at + T::CE <= nr ? 0 : at + T::CE - nr;        // elements to start earlier
+                    __builtin_memcpy(&st[i], base + (long long)off[i] - back * T::E, 16);
+                    st[i] = move_down(st[i], TR ? down[i % (TR ? N : 1)] : back * T::E);
+                }
+            }
         } else {
             const long long rows = TR ? reds : outs, cols = TR ? outs : reds;
 #pragma unroll
-            for (int i = 0; i < T::CH; ++i) {
-                const int L = i * NT + tid;
-                const int row = T::row_of(L), col = T::col_of(L);
+            for (int i = 0; i < N; ++i) {
+                const int row = row_of(i, tid), col = col_of(i, tid);
                 uint4 v = make_uint4(0, 0, 0, 0);
                 if (row < rows && col < cols) {
                     const char* p = base + (row * ld + col) * T::E;
@@ -422,9 +475,9 @@ struct Loader {
         }
     }
     __device__ __forceinline__ void put(unsigned char* tile, int tid) {
-        if constexpr (!DMA) {
+        if constexpr (WAY == REGS) {
 #pragma unroll
-            for (int i = 0; i < T::CH; ++i) *reinterpret_cast<uint4*>(tile + (i * NT + tid) * 16) = st[i];
+            for (int i = 0; i < N; ++i) *reinterpret_cast<uint4*>(tile + (i * NT + tid) * 16) = st[i];
         }
     }
 };
@@ -433,13 +486,14 @@ template <int WP, int WQ>
 __host__ __device__ constexpr int epi_bytes() { return 16 * (WQ + 4) * 4; }
 
 // BP x BQ of C per workgroup of WVP x WVQ waves.
-template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, bool DMA>
+template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
 __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     constexpr int NT = WVP * WVQ * 64;
     constexpr int TA = LAY == DW, TB = LAY != FWD;
     constexpr int WP = BP / WVP, WQ = BQ / WVQ, FP = WP / 16, FQ = WQ / 16;
-    using LA = Loader<DT, TA, BP, NT, DMA>;
-    using LB = Loader<DT, TB, BQ, NT, DMA>;
+    using LA = Loader<DT, TA, BP, NT, WAY>;
+    using LB = Loader<DT, TB, BQ, NT, WAY>;
+    constexpr bool DMA = WAY != REGS;
     using TAt = typename LA::T;
     using TBt = typename LB::T;
     constexpr int BK = TAt::BK, E = TAt::E;
@@ -480,8 +534,8 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
         const long long r = (long long)(s ? kt - nt0 : kt) * BK, left = red[s] - r, ra = r_lo + r;
         const char* pa = reinterpret_cast<const char*>(sg.a) + (TA ? ra * sg.lda + p0 : p0 * sg.lda + ra) * E;
         const char* pb = reinterpret_cast<const char*>(sg.b) + (TB ? ra * sg.ldb + q0 : q0 * sg.ldb + ra) * E;
-        la.fetch(pa, sg.lda, g.P - p0, left, tid, lds0 + buf * STAGE);
-        lb.fetch(pb, sg.ldb, g.Q - q0, left, tid, lds0 + buf * STAGE + TAt::BYTES);
+        la.fetch(pa, sg.lda, g.P - p0, ra, left, tid, lds0 + buf * STAGE);
+        lb.fetch(pb, sg.ldb, g.Q - q0, ra, left, tid, lds0 + buf * STAGE + TAt::BYTES);
     };
     la.start(g.seg[0].lda, g.P - p0, tid);
     lb.start(g.seg[0].ldb, g.Q - q0, tid);
@@ -614,13 +668,13 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     }
 }
 
-template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, bool DMA>
+template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
 int launch(GemmArgs& g, hipStream_t s) {
     const long long tp = (g.P + BP - 1) / BP, tq = (g.Q + BQ - 1) / BQ;
     NERF_REQUIRE(tp * tq < (1ll << 31), "linear: %lld x %lld outputs are too many for one launch", g.P, g.Q);
     g.tiles_p = (unsigned)tp;
     g.tiles_q = (unsigned)tq;
-    auto k = gemm_kernel<DT, LAY, BP, BQ, WVP, WVQ, DMA>;
+    auto k = gemm_kernel<DT, LAY, BP, BQ, WVP, WVQ, WAY>;
     hipLaunchKernelGGL(k, dim3((unsigned)(tp * tq), g.splits), dim3(WVP * WVQ * 64), 0, s, g);
     NERF_LAUNCH_CHECK();
     return NERF_OK;

@@ -1,6 +1,6 @@
 // Which tile a product of linear.h runs on.
 #pragma once
-#include "linear.h"
+#include "linear_rows.h"
 
 namespace nerf {
 namespace lin {
@@ -27,12 +27,15 @@ template <int DT, int LAY>
 int gemm_tiles(GemmArgs& g, hipStream_t s) {
     auto tiles = [&](int n) { return ((g.P + n - 1) / n) * ((g.Q + n - 1) / n) * g.splits; };
     if (dma_ok<DT>(LAY, g)) {
-        if (LAY == FWD && DT != F8W && tiles(256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, true>(g, s);
-        if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, true>(g, s);
-        return launch<DT, LAY, 64, 64, 2, 2, true>(g, s);
+        if constexpr (LAY != DW && elem_size(DT) == 2) {
+            if (g.nseg == 1 && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (g.Q <= 128 || g.seg[0].red <= 128 ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
+        }
+        if (LAY == FWD && DT != F8W && tiles(256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, DMA16>(g, s);
+        if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, DMA16>(g, s);
+        return launch<DT, LAY, 64, 64, 2, 2, DMA16>(g, s);
     }
-    if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, false>(g, s);
-    return launch<DT, LAY, 64, 64, 2, 2, false>(g, s);
+    if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, REGS>(g, s);
+    return launch<DT, LAY, 64, 64, 2, 2, REGS>(g, s);
 }
 
 template <int DT>
