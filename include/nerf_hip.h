@@ -305,16 +305,23 @@ int nerf_adam_step(int n_tensors, float* const* params_host, const float* const*
  * [x0 | x1 [M,k1]] side by side (the concatenation behind a skip connection, never formed); w [N, k0+k1] as nn.Linear
  * holds it; bias [N] or NULL; residual [M,N] or NULL.  z [M,N] or NULL receives the argument of act, which the
  * backward needs (for relu without a residual y itself serves).  M < 2^31, N and k up to 2^24.                       */
+/* workspace: nerf_linear_workspace_bytes(...) bytes (often 0: the copies of badly aligned operands that many outputs
+ * use, the parts of a long reduction with few outputs) on a 256-byte boundary, not shared with a call that may run at the
+ * same time.                                                                                                         */
+size_t nerf_linear_workspace_bytes(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
+                                   const void* w, long long ldw, long long M, int N);
 int nerf_linear(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
                 const void* w, long long ldw, const void* bias, int activation, const void* residual, long long ldr,
-                void* y, long long ldy, void* z, long long ldz, long long M, int N, void* stream);
+                void* y, long long ldy, void* z, long long ldz, long long M, int N, void* workspace,
+                size_t workspace_bytes, void* stream);
 
 /* Gradients of nerf_linear for g [M,N] = dL/dy (the residual's gradient is g itself).  z as the forward wrote it (not
  * read for NERF_ACT_NONE).  dx0 [M,k0], dx1 [M,k1], dw [N,k0+k1] contiguous and db [N] are overwritten; each may be
  * NULL and is then not computed (x0, x1 are read for dw only, w for dx0 and dx1 only).  With M = 0 dw and db are
- * zeros.  workspace: nerf_linear_backward_workspace_bytes(...) bytes on a 256-byte boundary, not shared with a call
- * that may run at the same time.                                                                                     */
-size_t nerf_linear_backward_workspace_bytes(int dtype, long long M, int N, int k0, int k1, int activation);
+ * zeros.  workspace: as for nerf_linear, nerf_linear_backward_workspace_bytes(...) bytes.                            */
+size_t nerf_linear_backward_workspace_bytes(int dtype, const void* g, long long ldg, int activation, const void* x0,
+                                            long long ldx0, int k0, const void* x1, long long ldx1, int k1, const void* w,
+                                            long long ldw, int want_dx0, int want_dx1, int want_dw, long long M, int N);
 int nerf_linear_backward(int dtype, const void* g, long long ldg, const void* z, long long ldz, int activation,
                          const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
                          const void* w, long long ldw, void* dx0, long long lddx0, void* dx1, long long lddx1,
@@ -322,9 +329,11 @@ int nerf_linear_backward(int dtype, const void* g, long long ldg, const void* z,
 
 /* nerf_linear on 8-bit operands (e4m3: four exponent bits, no infinities, largest 448): xq [M,K] and wq [N,K] hold
  * numbers that stand for x_scale[m] xq and w_scale[n] wq.  y, bias and residual are of type out_dtype.               */
+size_t nerf_linear_q8_workspace_bytes(const void* xq, long long ldx, const void* wq, long long ldw, long long M, int N, int K);
 int nerf_linear_q8(const void* xq, long long ldx, const float* x_scale, const void* wq, long long ldw,
                    const float* w_scale, int out_dtype, const void* bias, int activation, const void* residual,
-                   long long ldr, void* y, long long ldy, long long M, int N, int K, void* stream);
+                   long long ldr, void* y, long long ldy, long long M, int N, int K, void* workspace,
+                   size_t workspace_bytes, void* stream);
 
 /* h = x + residual (residual NULL: h = x), y = w h / sqrt(mean(h^2) + eps) over the N columns of each row.  The sum and
  * the norm are taken in float32 before h is rounded to dtype.  Exactly one of y [M,N] and q is given: q [M,N] holds y in

@@ -34,6 +34,7 @@ struct Seg {
     const void *a, *b;
     long long lda, ldb;          // elements between rows of the operand as it lies in memory
     long long red;               // length of the reduction over this piece
+    bool a_padded, b_padded;     // rows go on with zeros to a whole number of 16-byte chunks
 };
 
 struct GemmArgs {
@@ -52,6 +53,17 @@ struct GemmArgs {
     int out_dt;                  // type of y, bias, res, z
     unsigned tiles_p, tiles_q;
 };
+
+// A product of few tiles and a long reduction is cut until about 256 workgroups of 64 x 64 have work, each with four
+// k-tiles at least; linear.hip adds the parts up and runs the epilogue on the sums.  (73 x 409 x 3280 float32: 86 us in
+// one part.)
+inline int splits_for(long long P, long long Q, long long red, int elem) {
+    const long long tiles = ((P + 63) / 64) * ((Q + 63) / 64), k_tiles = (red * elem + 127) / 128;
+    if (tiles > 128 || k_tiles < 8) return 1;
+    const long long s = 256 / tiles < k_tiles / 4 ? 256 / tiles : k_tiles / 4;
+    return s < 1 ? 1 : (int)s;
+}
+constexpr long long FEW_ROWS = 64;       // up to here few_rows_kernel takes the forward product
 
 // what the three products need of the operands' layouts
 enum Layout { FWD = 0, DX = 1, DW = 2 };

@@ -1,5 +1,7 @@
 // C entry points of the linear layers, and the passes around their products: the gradient through the activation with
 // the bias gradient's column sums, and the sums over the parts of a split reduction.
+#include <algorithm>
+
 #include "linear.h"
 
 namespace nerf {
@@ -11,8 +13,10 @@ namespace lin {
 struct ActGradArgs {
     const void *g, *z;
     long long ldg, ldz;
-    void* gz;                    // [M][N] or null
+    void* gz;                    // [M][ldgz] or null: N columns and zeros behind them
+    long long ldgz;
     float* colsum;               // [blocks][N] or null
+    void* db;                    // [N]: the sums themselves, where one block holds all samples; or null
     long long M, N, rows;
     int act;
 };
@@ -35,7 +39,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) g[j] *= act_grad(z[j], a.act);
                 }
-                if (a.gz) st8<DT>(a.gz, p * a.N + q, g);
+                if (a.gz) st8<DT>(a.gz, p * a.ldgz + q, g);
             } else {
 #pragma unroll
                 for (int j = 0; j < 8; ++j) {
@@ -43,15 +47,15 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
                     if (q + j < a.N) {
                         g[j] = ld_elem(a.g, p * a.ldg + q + j, DT);
                         if (a.act != NERF_ACT_NONE) g[j] *= act_grad(ld_elem(a.z, p * a.ldz + q + j, DT), a.act);
-                        if (a.gz) st_elem(a.gz, p * a.N + q + j, g[j], DT);
                     }
+                    if (a.gz && q + j < a.ldgz) st_elem(a.gz, p * a.ldgz + q + j, g[j], DT);
                 }
             }
 #pragma unroll
             for (int j = 0; j < 8; ++j) sum[j] += g[j];
         }
     }
-    if (!a.colsum) return;
+    if (!a.colsum && !a.db) return;
 #pragma unroll
     for (int j = 0; j < 8; ++j) part[ty][tx * 8 + j] = sum[j];
     __syncthreads();
@@ -60,7 +64,10 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
         float s = 0.f;
 #pragma unroll
         for (int r = 0; r < 32; ++r) s += part[r][threadIdx.x];
-        if (c < a.N) a.colsum[(long long)blockIdx.y * a.N + c] = s;
+        if (c < a.N) {
+            if (a.db) st_elem(a.db, c, s, DT);
+            else a.colsum[(long long)blockIdx.y * a.N + c] = s;
+        }
     }
 }
 
@@ -115,21 +122,177 @@ int part_sum(int dtype, const float* parts, int n, long long rows, long long col
     return NERF_OK;
 }
 
+// The epilogue on the sums of a split product: one thread adds eight columns' parts, in order.
+template <int DT>
+__global__ void __launch_bounds__(256) finish_kernel(const GemmArgs g, int parts) {
+    const long long groups = (g.Q + 7) / 8, t = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long p = t / groups, q = t % groups * 8;
+    if (p >= g.P) return;
+    const bool whole = q + 8 <= g.Q;
+    const int n = whole ? 8 : (int)(g.Q - q);
+    float v[8] = {};
+    for (int k = 0; k < parts; ++k) {
+        float t8[8];
+        some8<F32>(g.partial, ((long long)k * g.P + p) * g.Q + q, whole, n, t8, F32);
+#pragma unroll
+        for (int j = 0; j < 8; ++j) v[j] += t8[j];
+    }
+    epilogue8<DT>(g, p, q, v);
+}
+
+// Rows copied to places on 16 bytes, zeros behind their ends to a whole chunk.  One chunk a thread.
+template <int E>
+__global__ void __launch_bounds__(256) pack_kernel(const char* src, long long ld, long long rows, long long cols, uint4* dst, long long chunks) {
+    constexpr int CE = 16 / E;
+    const long long t = (long long)blockIdx.x * 256 + threadIdx.x, row = t / chunks, c = t % chunks * CE;
+    if (row >= rows) return;
+    uint4 v;
+    const char* p = src + (row * ld + c) * E;
+    if (c + CE <= cols) __builtin_memcpy(&v, p, 16);
+    else v = part_chunk<E>(p, (int)(cols - c));
+    dst[t] = v;
+}
+
 static int dispatch_gemm(int dtype, int layout, GemmArgs& g, hipStream_t s) {
-    g.out_dt = dtype;
+    if (dtype != F8) g.out_dt = dtype;
     switch (dtype) {
         case F32: return gemm_f32(layout, g, s);
         case BF16: return gemm_bf16(layout, g, s);
-        default: return gemm_f16(layout, g, s);
+        case F16: return gemm_f16(layout, g, s);
+        default: return gemm_f8(g, s);
     }
 }
 
-// Column sums: about 512 blocks of samples, at least 64 samples each.
+static size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+
+// A matrix as a product reads it, and where its packed copy goes if it needs one.
+struct Mat {
+    const void* p;
+    long long ld, rows, cols;
+    bool padded;
+};
+// Rows on 16 bytes, and whole chunks
+static bool dma_rows(const Mat& m, int e) { return ((uintptr_t)m.p & 15) == 0 && (m.ld * e) % 16 == 0 && (m.padded || (m.cols * e) % 16 == 0); }
+static long long packed_ld(long long cols, int e) { return (cols * e + 15) / 16 * 16 / e; }
+static size_t packed_bytes(const Mat& m, int e) { return align256((size_t)m.rows * packed_ld(m.cols, e) * e); }
+static int pack(Mat& m, int e, char* to, hipStream_t s) {
+    const long long ldd = packed_ld(m.cols, e), chunks = ldd * e / 16;
+    const dim3 grid((unsigned)((m.rows * chunks + 255) / 256));
+    const char* src = static_cast<const char*>(m.p);
+    uint4* dst = reinterpret_cast<uint4*>(to);
+    if (e == 4) hipLaunchKernelGGL(pack_kernel<4>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
+    else if (e == 2) hipLaunchKernelGGL(pack_kernel<2>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
+    else hipLaunchKernelGGL(pack_kernel<1>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
+    NERF_LAUNCH_CHECK();
+    m.p = to;
+    m.ld = ldd;
+    m.padded = true;
+    return NERF_OK;
+}
+
+// One product with its copies and its split: what it takes of the workspace, and the launches.
+struct Product {
+    int dtype, layout;
+    Mat a[2], b[2];
+    int nseg;
+    long long P, Q;
+    long long red[2];
+    bool can_split;
+
+    // Unaligned rows cost a product about its own time over in the forward layout (each row's lines come twice; 0.4 times in
+    // float32), four times it where an operand lies reduction-major; a copy costs its bytes both ways and a launch.
+    // Measured: 4096 x 4096 x 4095 bf16 308 us as it lies, 151 us copied; 4097 x 515 x 1021 fp16 forward 23 and 31 us,
+    // dW 67 and 39 us.
+    bool packs() const {
+        const int e = elem_size(dtype);
+        double copy_us = 0, products = 0;
+        for (int s = 0; s < nseg; ++s) {
+            products += (double)P * Q * red[s];
+            for (const Mat& m : {a[s], b[s]}) {
+                if (m.rows >= (1ll << 31) || m.cols * e >= (1ll << 22)) return false;
+                if (!dma_rows(m, e)) copy_us += 4 + (double)m.rows * m.cols * e * 2 / 5e6;
+            }
+        }
+        if (copy_us == 0 || (layout == FWD && P <= FEW_ROWS)) return false;
+        const double aligned_us = products * 2 / (dtype == F32 ? 130e6 : 700e6);
+        return copy_us < aligned_us * (dtype == F32 ? 0.4 : layout == FWD ? 1 : 4);
+    }
+    int splits() const {
+        if (!can_split || nseg != 1 || (layout == FWD && P <= FEW_ROWS)) return 1;
+        return splits_for(P, Q, red[0], elem_size(dtype));
+    }
+    size_t bytes() const {
+        size_t n = 0;
+        if (packs())
+            for (int s = 0; s < nseg; ++s)
+                for (const Mat& m : {a[s], b[s]})
+                    if (!dma_rows(m, elem_size(dtype))) n += packed_bytes(m, elem_size(dtype));
+        if (splits() > 1) n += align256((size_t)splits() * P * Q * 4);
+        return n;
+    }
+    // given: parts that the caller has set up and will add up itself (g.partial, g.red_part)
+    int run(GemmArgs& g, char* ws, hipStream_t st, int given = 1) {
+        const int e = elem_size(dtype), sp = splits();
+        if (packs())
+            for (int s = 0; s < nseg; ++s)
+                for (Mat* m : {&a[s], &b[s]})
+                    if (!dma_rows(*m, e)) {
+                        const size_t n = packed_bytes(*m, e);
+                        const int rc = pack(*m, e, ws, st);
+                        if (rc != NERF_OK) return rc;
+                        ws += n;
+                    }
+        for (int s = 0; s < nseg; ++s) g.seg[s] = {a[s].p, b[s].p, a[s].ld, b[s].ld, red[s], a[s].padded, b[s].padded};
+        g.nseg = nseg;
+        g.P = P;
+        g.Q = Q;
+        g.splits = given;
+        if (sp == 1) return dispatch_gemm(dtype, layout, g, st);
+        const long long unit = 128;              // a multiple of every type's k-tile
+        g.red_part = ((red[0] + sp - 1) / sp + unit - 1) / unit * unit;
+        g.splits = (int)((red[0] + g.red_part - 1) / g.red_part);
+        g.partial = reinterpret_cast<float*>(ws);
+        int rc = dispatch_gemm(dtype, layout, g, st);
+        if (rc != NERF_OK) return rc;
+        const dim3 grid((unsigned)((P * ((Q + 7) / 8) + 255) / 256));
+        switch (dtype) {
+            case F32: hipLaunchKernelGGL(finish_kernel<F32>, grid, dim3(256), 0, st, g, g.splits); break;
+            case BF16: hipLaunchKernelGGL(finish_kernel<BF16>, grid, dim3(256), 0, st, g, g.splits); break;
+            case F16: hipLaunchKernelGGL(finish_kernel<F16>, grid, dim3(256), 0, st, g, g.splits); break;
+            default: hipLaunchKernelGGL(finish_kernel<F8>, grid, dim3(256), 0, st, g, g.splits); break;
+        }
+        NERF_LAUNCH_CHECK();
+        return NERF_OK;
+    }
+};
+
+static Product forward_product(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
+                               const void* w, long long ldw, long long M, int N) {
+    const int e = elem_size(dtype);
+    Product f = {};
+    f.dtype = dtype;
+    f.layout = FWD;
+    f.nseg = k1 > 0 ? 2 : 1;
+    f.a[0] = {x0, ldx0, M, k0, false};
+    f.a[1] = {x1, ldx1, M, k1, false};
+    f.b[0] = {w, ldw, N, k0, false};
+    f.b[1] = {static_cast<const char*>(w) + (size_t)k0 * e, ldw, N, k1, false};
+    f.P = M;
+    f.Q = N;
+    f.red[0] = k0;
+    f.red[1] = k1;
+    f.can_split = true;
+    return f;
+}
+
+// Column sums: about 512 blocks of samples, at least 64 samples each; up to 256 samples one block that writes db itself,
+// a launch less where launches are the time.
 static long long colsum_rows(long long M) {
+    if (M <= 256) return M;
     const long long r = (M + 511) / 512;
     return r < 64 ? 64 : r;
 }
-static int colsum_blocks(long long M) { return (int)((M + colsum_rows(M) - 1) / colsum_rows(M)); }
+static int colsum_blocks(long long M) { return M ? (int)((M + colsum_rows(M) - 1) / colsum_rows(M)) : 0; }
 
 // dW = gz^T x has a long reduction (the samples) and few outputs: cut until about 512 workgroups of 128 x 128 have work,
 // not below 512 samples a part.
@@ -141,24 +304,63 @@ static int dw_splits(long long M, long long N, long long K) {
     return s < 1 ? 1 : (int)s;
 }
 
-static size_t align256(size_t b) { return (b + 255) & ~(size_t)255; }
+// The backward pass: gz where the layer has an activation, the column sums' parts, then scratch of one product at a time
+// (its copies, the parts of dW).
+struct Backward {
+    int dtype, act;
+    long long M, N, k[2];
+    const void *g, *x[2], *w;
+    long long ldg, ldx[2], ldw;
 
-struct Workspace {
-    size_t gz, colsum, partial, all;
-};
-static Workspace backward_workspace(int dtype, long long M, long long N, long long k0, long long k1, int act) {
-    Workspace w;
-    w.gz = 0;
-    w.colsum = act == NERF_ACT_NONE ? 0 : align256((size_t)M * N * elem_size(dtype));
-    w.partial = w.colsum + align256((size_t)colsum_blocks(M) * N * 4);
-    size_t part = 0;
-    for (long long k : {k0, k1}) {
-        const int sp = k > 0 ? dw_splits(M, N, k) : 1;
-        if (sp > 1 && (size_t)sp * N * k * 4 > part) part = (size_t)sp * N * k * 4;
+    bool through() const { return act != NERF_ACT_NONE; }
+    long long ldgz() const { return packed_ld(N, elem_size(dtype)); }
+    size_t colsum_at() const { return through() ? align256((size_t)M * ldgz() * elem_size(dtype)) : 0; }
+    size_t scratch_at() const { return colsum_at() + align256((size_t)colsum_blocks(M) * N * 4); }
+    Mat gz(char* ws) const {
+        if (through()) return {ws, ldgz(), M, N, true};
+        return {g, ldg, M, N, false};
     }
-    w.all = w.partial + align256(part);
-    return w;
-}
+    Product dx(int piece, char* ws) const {
+        Product f = {};
+        f.dtype = dtype;
+        f.layout = DX;
+        f.nseg = 1;
+        f.a[0] = gz(ws);
+        f.b[0] = {static_cast<const char*>(w) + (piece ? (size_t)k[0] * elem_size(dtype) : 0), ldw, N, k[piece], false};
+        f.P = M;
+        f.Q = k[piece];
+        f.red[0] = N;
+        f.can_split = true;
+        return f;
+    }
+    Product dw(int piece, char* ws) const {
+        Product f = {};
+        f.dtype = dtype;
+        f.layout = DW;
+        f.nseg = 1;
+        f.a[0] = gz(ws);
+        f.b[0] = {x[piece], ldx[piece], M, k[piece], false};
+        f.P = N;
+        f.Q = k[piece];
+        f.red[0] = M;
+        return f;
+    }
+    // the parts of dW stand behind its copies
+    size_t dw_parts(int piece) const {
+        const int s = dw_splits(M, N, k[piece]);
+        return s > 1 ? align256((size_t)s * N * k[piece] * 4) : 0;
+    }
+    size_t bytes(bool want_x0, bool want_x1, bool want_w) const {
+        size_t n = 0;
+        char* ws = nullptr;
+        for (int piece = 0; piece < 2; ++piece) {
+            if (k[piece] == 0) continue;
+            if (piece ? want_x1 : want_x0) n = std::max(n, dx(piece, ws).bytes());
+            if (want_w) n = std::max(n, dw(piece, ws).bytes() + dw_parts(piece));
+        }
+        return scratch_at() + n;
+    }
+};
 
 static bool dtype_ok(int d) { return d == F32 || d == BF16 || d == F16; }
 static bool act_ok(int a) { return a >= NERF_ACT_NONE && a <= NERF_ACT_SILU; }
@@ -166,6 +368,10 @@ static bool act_ok(int a) { return a >= NERF_ACT_NONE && a <= NERF_ACT_SILU; }
 constexpr long long MAX_DIM = 1ll << 24;       // inputs and outputs of a layer
 constexpr long long MAX_ROWS = 1ll << 31;
 
+#define NERF_LINEAR_WORKSPACE(who, need)                                                                                \
+    NERF_REQUIRE(workspace_bytes >= (need) && ((need) == 0 || workspace), who ": workspace of %zu bytes, %zu needed",   \
+                 workspace_bytes, (size_t)(need));                                                                      \
+    NERF_REQUIRE(((uintptr_t)workspace & 255) == 0, who ": the workspace must start on 256 bytes")
 #define NERF_LINEAR_SIZES(who)                                                                                          \
     NERF_REQUIRE(M >= 0 && M < MAX_ROWS && N >= 1 && N <= MAX_DIM, who ": bad sizes M=%lld N=%d", M, N);              \
     NERF_REQUIRE(k0 >= 1 && k0 <= MAX_DIM && k1 >= 0 && k1 <= MAX_DIM, who ": bad input widths %d, %d", k0, k1)
@@ -176,9 +382,16 @@ constexpr long long MAX_ROWS = 1ll << 31;
 using namespace nerf;
 using namespace nerf::lin;
 
+extern "C" size_t nerf_linear_workspace_bytes(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1,
+                                              int k1, const void* w, long long ldw, long long M, int N) {
+    if (!dtype_ok(dtype) || M < 0 || M >= MAX_ROWS || N < 1 || N > MAX_DIM || k0 < 1 || k0 > MAX_DIM || k1 < 0 || k1 > MAX_DIM) return 0;
+    return forward_product(dtype, x0, ldx0, k0, x1, ldx1, k1, w, ldw, M, N).bytes();
+}
+
 extern "C" int nerf_linear(int dtype, const void* x0, long long ldx0, int k0, const void* x1, long long ldx1, int k1,
                            const void* w, long long ldw, const void* bias, int activation, const void* residual,
-                           long long ldr, void* y, long long ldy, void* z, long long ldz, long long M, int N, void* stream) {
+                           long long ldr, void* y, long long ldy, void* z, long long ldz, long long M, int N,
+                           void* workspace, size_t workspace_bytes, void* stream) {
     NERF_REQUIRE(dtype_ok(dtype), "nerf_linear: unknown type %d", dtype);
     NERF_REQUIRE(act_ok(activation), "nerf_linear: unknown activation %d", activation);
     NERF_LINEAR_SIZES("nerf_linear");
@@ -186,14 +399,9 @@ extern "C" int nerf_linear(int dtype, const void* x0, long long ldx0, int k0, co
     NERF_REQUIRE(x0 && w && y && (k1 == 0 || x1), "nerf_linear: null pointer");
     NERF_REQUIRE(ldx0 >= k0 && (k1 == 0 || ldx1 >= k1) && ldw >= (long long)k0 + k1 && ldy >= N && (!residual || ldr >= N) && (!z || ldz >= N),
                  "nerf_linear: a row stride is below its row's length");
-    const int e = elem_size(dtype);
+    Product f = forward_product(dtype, x0, ldx0, k0, x1, ldx1, k1, w, ldw, M, N);
+    NERF_LINEAR_WORKSPACE("nerf_linear", f.bytes());
     GemmArgs g = {};
-    g.seg[0] = {x0, w, ldx0, ldw, k0};
-    g.seg[1] = {x1, static_cast<const char*>(w) + (size_t)k0 * e, ldx1, ldw, k1};
-    g.nseg = k1 > 0 ? 2 : 1;
-    g.P = M;
-    g.Q = N;
-    g.splits = 1;
     g.bias = bias;
     g.res = residual;
     g.y = y;
@@ -202,12 +410,19 @@ extern "C" int nerf_linear(int dtype, const void* x0, long long ldx0, int k0, co
     g.ldy = ldy;
     g.ldz = ldz;
     g.act = activation;
-    return dispatch_gemm(dtype, FWD, g, as_stream(stream));
+    g.out_dt = dtype;
+    return f.run(g, static_cast<char*>(workspace), as_stream(stream));
+}
+
+extern "C" size_t nerf_linear_q8_workspace_bytes(const void* xq, long long ldx, const void* wq, long long ldw, long long M, int N, int K) {
+    if (M < 0 || M >= MAX_ROWS || N < 1 || N > MAX_DIM || K < 1 || K > MAX_DIM) return 0;
+    return forward_product(F8, xq, ldx, K, nullptr, 0, 0, wq, ldw, M, N).bytes();
 }
 
 extern "C" int nerf_linear_q8(const void* xq, long long ldx, const float* x_scale, const void* wq, long long ldw,
                               const float* w_scale, int out_dtype, const void* bias, int activation, const void* residual,
-                              long long ldr, void* y, long long ldy, long long M, int N, int K, void* stream) {
+                              long long ldr, void* y, long long ldy, long long M, int N, int K, void* workspace,
+                              size_t workspace_bytes, void* stream) {
     NERF_REQUIRE(dtype_ok(out_dtype), "nerf_linear_q8: unknown type %d", out_dtype);
     NERF_REQUIRE(act_ok(activation), "nerf_linear_q8: unknown activation %d", activation);
     const int k0 = K, k1 = 0;
@@ -215,12 +430,9 @@ extern "C" int nerf_linear_q8(const void* xq, long long ldx, const float* x_scal
     if (M == 0) return NERF_OK;
     NERF_REQUIRE(xq && wq && x_scale && w_scale && y, "nerf_linear_q8: null pointer");
     NERF_REQUIRE(ldx >= K && ldw >= K && ldy >= N && (!residual || ldr >= N), "nerf_linear_q8: a row stride is below its row's length");
+    Product f = forward_product(F8, xq, ldx, K, nullptr, 0, 0, wq, ldw, M, N);
+    NERF_LINEAR_WORKSPACE("nerf_linear_q8", f.bytes());
     GemmArgs g = {};
-    g.seg[0] = {xq, wq, ldx, ldw, K};
-    g.nseg = 1;
-    g.P = M;
-    g.Q = N;
-    g.splits = 1;
     g.bias = bias;
     g.res = residual;
     g.y = y;
@@ -230,14 +442,22 @@ extern "C" int nerf_linear_q8(const void* xq, long long ldx, const float* x_scal
     g.sq = w_scale;
     g.act = activation;
     g.out_dt = out_dtype;
-    return gemm_f8(g, as_stream(stream));
+    return f.run(g, static_cast<char*>(workspace), as_stream(stream));
 }
 
-extern "C" size_t nerf_linear_backward_workspace_bytes(int dtype, long long M, int N, int k0, int k1, int activation) {
+static Backward backward_of(int dtype, int activation, const void* g, long long ldg, const void* x0, long long ldx0, int k0,
+                            const void* x1, long long ldx1, int k1, const void* w, long long ldw, long long M, int N) {
+    return {dtype, activation, M, N, {k0, k1}, g, {x0, x1}, w, ldg, {ldx0, ldx1}, ldw};
+}
+
+extern "C" size_t nerf_linear_backward_workspace_bytes(int dtype, const void* g, long long ldg, int activation, const void* x0,
+                                                       long long ldx0, int k0, const void* x1, long long ldx1, int k1,
+                                                       const void* w, long long ldw, int want_dx0, int want_dx1, int want_dw,
+                                                       long long M, int N) {
     if (!dtype_ok(dtype) || !act_ok(activation) || M < 0 || M >= MAX_ROWS || N < 1 || N > MAX_DIM || k0 < 1 || k0 > MAX_DIM ||
         k1 < 0 || k1 > MAX_DIM)
         return 0;
-    return backward_workspace(dtype, M, N, k0, k1, activation).all;
+    return backward_of(dtype, activation, g, ldg, x0, ldx0, k0, x1, ldx1, k1, w, ldw, M, N).bytes(want_dx0, want_dx1, want_dw);
 }
 
 extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, const void* z, long long ldz, int activation,
@@ -263,23 +483,24 @@ extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, con
     NERF_REQUIRE(ldg >= N && (activation == NERF_ACT_NONE || ldz >= N) && (!dw || (ldx0 >= k0 && (k1 == 0 || ldx1 >= k1))) &&
                      (!w || ldw >= K) && (!dx0 || lddx0 >= k0) && (!dx1 || lddx1 >= k1),
                  "nerf_linear_backward: a row stride is below its row's length");
-    const Workspace ws = backward_workspace(dtype, M, N, k0, k1, activation);
-    NERF_REQUIRE(workspace_bytes >= ws.all && (ws.all == 0 || workspace), "nerf_linear_backward: workspace of %zu bytes, %zu needed",
-                 workspace_bytes, ws.all);
-    NERF_REQUIRE(((uintptr_t)workspace & 255) == 0, "nerf_linear_backward: the workspace must start on 256 bytes");
+    const Backward bw = backward_of(dtype, activation, g, ldg, x0, ldx0, k0, x1, ldx1, k1, w, ldw, M, N);
+    NERF_LINEAR_WORKSPACE("nerf_linear_backward", bw.bytes(dx0 != nullptr, dx1 != nullptr, dw != nullptr));
     char* base = static_cast<char*>(workspace);
     const int e = elem_size(dtype);
 
-    const bool through = activation != NERF_ACT_NONE && (dx0 || dx1 || dw);
-    float* colsum = reinterpret_cast<float*>(base + ws.colsum);
+    const bool through = bw.through() && (dx0 || dx1 || dw);
+    float* colsum = reinterpret_cast<float*>(base + bw.colsum_at());
     if (through || db) {
         ActGradArgs a = {};
         a.g = g;
         a.z = z;
         a.ldg = ldg;
         a.ldz = ldz;
-        a.gz = through ? base + ws.gz : nullptr;
-        a.colsum = db ? colsum : nullptr;
+        a.gz = through ? base : nullptr;
+        a.ldgz = bw.ldgz();
+        const bool one = colsum_blocks(M) == 1;
+        a.colsum = db && !one ? colsum : nullptr;
+        a.db = one ? db : nullptr;
         a.M = M;
         a.N = N;
         a.rows = colsum_rows(M);
@@ -291,52 +512,40 @@ extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, con
             default: hipLaunchKernelGGL(act_grad_kernel<F16>, grid, dim3(256), 0, s, a); break;
         }
         NERF_LAUNCH_CHECK();
-        if (db) {
+        if (a.colsum) {
             const int rc = part_sum(dtype, colsum, colsum_blocks(M), 1, N, db, N, s);
             if (rc != NERF_OK) return rc;
         }
     }
-    const void* gz = through ? base + ws.gz : g;
-    const long long ldgz = through ? N : ldg;
 
     for (int piece = 0; piece < 2; ++piece) {
         const int k = piece ? k1 : k0;
         if (k == 0) continue;
-        const char* wp = static_cast<const char*>(w) + (piece ? (size_t)k0 * e : 0);
-        void* dx = piece ? dx1 : dx0;
-        if (dx) {
+        if (void* dx = piece ? dx1 : dx0) {
             GemmArgs a = {};
-            a.seg[0] = {gz, wp, ldgz, ldw, N};
-            a.nseg = 1;
-            a.P = M;
-            a.Q = k;
-            a.splits = 1;
             a.y = dx;
             a.ldy = piece ? lddx1 : lddx0;
-            const int rc = dispatch_gemm(dtype, DX, a, s);
+            const int rc = bw.dx(piece, base).run(a, base + bw.scratch_at(), s);
             if (rc != NERF_OK) return rc;
         }
         if (dw) {
+            Product f = bw.dw(piece, base);
             GemmArgs a = {};
-            a.seg[0] = {gz, piece ? x1 : x0, ldgz, piece ? ldx1 : ldx0, M};
-            a.nseg = 1;
-            a.P = N;
-            a.Q = k;
-            a.splits = dw_splits(M, N, k);
             char* out = static_cast<char*>(dw) + (piece ? (size_t)k0 * e : 0);
-            if (a.splits > 1) {
+            int sp = dw_splits(M, N, k);
+            if (sp > 1) {
                 const long long unit = 128;              // a multiple of every type's k-tile
-                a.red_part = ((M + a.splits - 1) / a.splits + unit - 1) / unit * unit;
-                a.splits = (int)((M + a.red_part - 1) / a.red_part);
-                a.partial = reinterpret_cast<float*>(base + ws.partial);
+                a.red_part = ((M + sp - 1) / sp + unit - 1) / unit * unit;
+                sp = (int)((M + a.red_part - 1) / a.red_part);
+                a.partial = reinterpret_cast<float*>(base + bw.scratch_at() + f.bytes());
             } else {
                 a.y = out;
                 a.ldy = K;
             }
-            int rc = dispatch_gemm(dtype, DW, a, s);
+            int rc = f.run(a, base + bw.scratch_at(), s, sp);
             if (rc != NERF_OK) return rc;
             if (a.partial) {
-                rc = part_sum(dtype, a.partial, a.splits, N, k, out, K, s);
+                rc = part_sum(dtype, a.partial, sp, N, k, out, K, s);
                 if (rc != NERF_OK) return rc;
             }
         }

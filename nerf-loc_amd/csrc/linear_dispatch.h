@@ -5,8 +5,9 @@
 namespace nerf {
 namespace lin {
 
-// LDS-DMA moves 16-byte chunks between 16-byte aligned places: rows of both operands have to start on 16 bytes, and no
-// chunk may hold the end of a row's valid part and something else (the zeros behind it are the loader's, chunk by chunk).
+// LDS-DMA moves 16-byte chunks between 16-byte aligned places: rows of both operands have to start on 16 bytes.  A chunk
+// that holds a row's end must hold zeros behind it where the row runs along the reduction (the neighbour's values would
+// be added); along C's rows or columns anything may follow, if it belongs to the buffer.
 template <int DT>
 inline bool dma_ok(int layout, const GemmArgs& g) {
     constexpr int E = elem_size(DT), CE = 16 / E;
@@ -15,10 +16,8 @@ inline bool dma_ok(int layout, const GemmArgs& g) {
         if (((uintptr_t)sg.a | (uintptr_t)sg.b) & 15) return false;
         if ((sg.lda * E) % 16 || (sg.ldb * E) % 16) return false;
         if (sg.lda * E * 256 >= (1ll << 31) || sg.ldb * E * 256 >= (1ll << 31)) return false;      // 32-bit offsets in a tile
-        const bool ta = layout == DW, tb = layout != FWD;
-        if ((!ta || !tb) && sg.red % CE) return false;
-        if (ta && g.P % CE) return false;
-        if (tb && g.Q % CE) return false;
+        const long long row_a = layout == DW ? g.P : sg.red, row_b = layout == FWD ? sg.red : g.Q;
+        if ((row_a % CE && !sg.a_padded) || (row_b % CE && !sg.b_padded)) return false;
     }
     return true;
 }
@@ -28,7 +27,7 @@ int gemm_tiles(GemmArgs& g, hipStream_t s) {
     auto tiles = [&](int n) { return ((g.P + n - 1) / n) * ((g.Q + n - 1) / n) * g.splits; };
     if (dma_ok<DT>(LAY, g)) {
         if constexpr (LAY != DW && elem_size(DT) == 2) {
-            if (g.nseg == 1 && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (g.Q <= 128 || g.seg[0].red <= 128 ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
+            if (g.nseg == 1 && !g.partial && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (g.Q <= 128 || g.seg[0].red <= 128 ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
         }
         if (LAY == FWD && DT != F8W && tiles(256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, DMA16>(g, s);
         if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, DMA16>(g, s);
@@ -42,7 +41,7 @@ template <int DT>
 int gemm_forward(GemmArgs& g, hipStream_t s) {
     if (g.P <= 16) return launch_few_rows<DT == F8 ? F8W : DT, 1>(g, s);
     if (g.P <= 32) return launch_few_rows<DT == F8 ? F8W : DT, 2>(g, s);
-    if (g.P <= 64) return launch_few_rows<DT == F8 ? F8W : DT, 4>(g, s);
+    if (g.P <= FEW_ROWS) return launch_few_rows<DT == F8 ? F8W : DT, 4>(g, s);
     return gemm_tiles<DT, FWD>(g, s);
 }
 

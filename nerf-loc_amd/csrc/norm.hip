@@ -29,6 +29,7 @@ struct NormGradArgs {
     const float* rstd;
     void* dx;
     float* dw_part;              // [blocks][N] or null
+    void* dw;                    // [N]: the sums themselves, where one workgroup has all rows; or null
     long long ldgy, ldgh, ldh, lddx, M;
     int N;
 };
@@ -206,13 +207,17 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_grad_kernel(cons
             if (live && c < a.N) put8<DT>(a.dx, row * a.lddx, c, a.N, g);
         }
     }
-    if (!a.dw_part) return;
+    if (!a.dw_part && !a.dw) return;
     if constexpr (ROWS == 1) {
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int c = (k * ROWT + t) * 8;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) if (c + j < a.N) a.dw_part[(long long)blockIdx.x * a.N + c + j] = dw[k][j];
+            for (int j = 0; j < 8; ++j) {
+                if (c + j >= a.N) continue;
+                if (a.dw) st_elem(a.dw, c + j, dw[k][j], DT);
+                else a.dw_part[(long long)blockIdx.x * a.N + c + j] = dw[k][j];
+            }
         }
     } else {
         constexpr int COLS = ROWT * VPT * 8;
@@ -224,7 +229,8 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_grad_kernel(cons
         for (int c = threadIdx.x; c < COLS && c < a.N; c += NT) {
             float s = 0.f;
             for (int r = 0; r < ROWS; ++r) s += sums[r * COLS + c];
-            a.dw_part[(long long)blockIdx.x * a.N + c] = s;
+            if (a.dw) st_elem(a.dw, c, s, DT);
+            else a.dw_part[(long long)blockIdx.x * a.N + c] = s;
         }
     }
 }
@@ -266,15 +272,19 @@ static int norm_launch(const NormArgs& a, hipStream_t s) {
     return NERF_OK;
 }
 template <int DT>
-static int norm_grad_launch(const NormGradArgs& a, void* dw, hipStream_t s) {
+static int norm_grad_launch(NormGradArgs a, void* dw, hipStream_t s) {
     const long long blocks = norm_grad_blocks(a.M, a.N);
+    if (blocks == 1) {
+        a.dw = dw;
+        a.dw_part = nullptr;
+    }
     if (blocks > 0) {
 #define NERF_CALL(T, V) hipLaunchKernelGGL((norm_grad_kernel<DT, T, V>), dim3((unsigned)blocks), dim3(T < 256 ? 256 : T), 0, s, a)
         NERF_NORM_SWITCH(a.N, NERF_CALL);
 #undef NERF_CALL
         NERF_LAUNCH_CHECK();
     }
-    return dw ? part_sum(DT, a.dw_part, (int)blocks, 1, a.N, dw, a.N, s) : NERF_OK;
+    return dw && blocks != 1 ? part_sum(DT, a.dw_part, (int)blocks, 1, a.N, dw, a.N, s) : NERF_OK;
 }
 
 }  // namespace lin
@@ -317,7 +327,7 @@ extern "C" int nerf_add_rms_norm_backward(int dtype, const void* gy, long long l
     NERF_REQUIRE(ldgy >= N && (!gh || ldgh >= N) && ldh >= N && (!dx || lddx >= N), "nerf_add_rms_norm_backward: a row stride is below its row's length");
     const size_t need = dw ? (size_t)norm_grad_blocks(M, N) * N * 4 : 0;
     NERF_REQUIRE(workspace_bytes >= need && (need == 0 || workspace), "nerf_add_rms_norm_backward: workspace of %zu bytes, %zu needed", workspace_bytes, need);
-    const NormGradArgs a = {gy, gh, h, w, rstd, dx, dw ? static_cast<float*>(workspace) : nullptr, ldgy, ldgh, ldh, lddx, M, N};
+    const NormGradArgs a = {gy, gh, h, w, rstd, dx, dw ? static_cast<float*>(workspace) : nullptr, nullptr, ldgy, ldgh, ldh, lddx, M, N};
     hipStream_t s = as_stream(stream);
     switch (dtype) {
         case F32: return norm_grad_launch<F32>(a, dw, s);

@@ -94,22 +94,31 @@ _SIGNATURES = {
                                       ctypes.POINTER(ctypes.c_longlong), ctypes.c_longlong, ctypes.c_float,
                                       ctypes.c_float, ctypes.c_float, ctypes.c_float, ctypes.c_float,
                                       ctypes.c_void_p]),
+    "nerf_linear_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
+                                                      ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
+                                                      ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int]),
     "nerf_linear": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
                                    ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                    ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
-                                   ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p]),
-    "nerf_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
-                                                               ctypes.c_int, ctypes.c_int]),
+                                   ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
+                                   ctypes.c_size_t, ctypes.c_void_p]),
+    "nerf_linear_backward_workspace_bytes": (ctypes.c_size_t, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
+                                                               ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
+                                                               ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int,
+                                                               ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_int,
+                                                               ctypes.c_int, ctypes.c_longlong, ctypes.c_int]),
     "nerf_linear_backward": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
                                             ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p,
                                             ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                             ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                             ctypes.c_void_p, ctypes.c_longlong, ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t,
                                             ctypes.c_void_p]),
+    "nerf_linear_q8_workspace_bytes": (ctypes.c_size_t, [ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
+                                                         ctypes.c_longlong, ctypes.c_int, ctypes.c_int]),
     "nerf_linear_q8": (ctypes.c_int, [ctypes.c_void_p, ctypes.c_longlong, _c_float_p, ctypes.c_void_p, ctypes.c_longlong,
                                       _c_float_p, ctypes.c_int, ctypes.c_void_p, ctypes.c_int, ctypes.c_void_p,
                                       ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_longlong, ctypes.c_int,
-                                      ctypes.c_int, ctypes.c_void_p]),
+                                      ctypes.c_int, ctypes.c_void_p, ctypes.c_size_t, ctypes.c_void_p]),
     "nerf_add_rms_norm": (ctypes.c_int, [ctypes.c_int, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong,
                                          ctypes.c_void_p, ctypes.c_float, ctypes.c_void_p, ctypes.c_longlong, ctypes.c_void_p,
                                          ctypes.c_longlong, ctypes.c_void_p, ctypes.c_longlong, _c_float_p, _c_float_p,
@@ -673,6 +682,7 @@ def adam_step(params, grads, exp_avgs, exp_avg_sqs, step, lr, beta1, beta2, eps,
 DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 ACTIVATIONS = {None: 0, "none": 0, "relu": 1, "gelu": 2, "silu": 3}
 NORM_MAX_WIDTH = 32768
+FEW_ROWS = 64            # up to here the forward products take no workspace
 
 
 _CALLS = {}
@@ -695,6 +705,11 @@ def _call(name, dev, *args):
 
 def _at(t):
     return None if t is None else t.data_ptr()
+
+
+def _scratch(nbytes, dev):
+    """Scratch of one call, its own every time: calls on other streams, or in captured graphs, may overlap."""
+    return torch.empty((nbytes,), dtype=torch.uint8, device=dev) if nbytes else None
 
 
 def activation_code(name):
@@ -771,8 +786,11 @@ def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)[:2]
     y = torch.empty((M, N), dtype=dt, device=dev)
     z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
-    _call("nerf_linear", dev, DTYPES[dt], _at(x0), ld0, k0, _at(x1), ld1, k1, _at(w), ldw, _at(b), act, _at(r), ldr,
-          _at(y), N, _at(z), N, M, N)
+    px, p1, pw = x0.data_ptr(), _at(x1), w.data_ptr()
+    nbytes = 0 if M <= FEW_ROWS else lib().nerf_linear_workspace_bytes(DTYPES[dt], px, ld0, k0, p1, ld1, k1, pw, ldw, M, N)
+    ws = _scratch(nbytes, dev)
+    _call("nerf_linear", dev, DTYPES[dt], px, ld0, k0, p1, ld1, k1, pw, ldw, _at(b), act, _at(r), ldr,
+          y.data_ptr(), N, _at(z), N, M, N, _at(ws), nbytes)
     return y, z
 
 
@@ -789,11 +807,12 @@ def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=Tru
     dx1 = new(M, k1) if want_x1 and x1 is not None else None
     dw = new(N, k0 + k1) if want_w else None
     db = new(N) if want_b else None
-    nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], M, N, k0, k1, act)
-    ws = torch.empty((nbytes,), dtype=torch.uint8, device=dev)      # its own in every call: calls on other streams may overlap
-    _call("nerf_linear_backward", dev, DTYPES[dt], _at(g), ldg, _at(zz), ldz, act, _at(x0), ld0, k0, _at(x1), ld1, k1,
-          _at(w), ldw, _at(dx0), k0, _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws),
-                                          nbytes)
+    pg, px, p1, pw = g.data_ptr(), x0.data_ptr(), _at(x1), w.data_ptr()
+    nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], pg, ldg, act, px, ld0, k0, p1, ld1, k1, pw, ldw,
+                                                        dx0 is not None, dx1 is not None, dw is not None, M, N)
+    ws = _scratch(nbytes, dev)
+    _call("nerf_linear_backward", dev, DTYPES[dt], pg, ldg, _at(zz), ldz, act, px, ld0, k0, p1, ld1, k1, pw, ldw, _at(dx0), k0,
+          _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws), nbytes)
     return dx0, dx1, dw, db
 
 
@@ -815,8 +834,11 @@ def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=Non
     b = None if bias is None else _vector(bias, "bias", N, out_dtype, dev)
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, out_dtype, dev)[:2]
     y = torch.empty((M, N), dtype=out_dtype, device=dev)
-    _call("nerf_linear_q8", dev, _at(xq), ldx, _at(xs), _at(wq), ldw, _at(ws), DTYPES[out_dtype], _at(b), act, _at(r),
-          ldr, _at(y), N, M, N, K)
+    px, pw = xq.data_ptr(), wq.data_ptr()
+    nbytes = 0 if M <= FEW_ROWS else lib().nerf_linear_q8_workspace_bytes(px, ldx, pw, ldw, M, N, K)
+    scratch = _scratch(nbytes, dev)
+    _call("nerf_linear_q8", dev, px, ldx, xs.data_ptr(), pw, ldw, ws.data_ptr(), DTYPES[out_dtype], _at(b), act, _at(r), ldr,
+          y.data_ptr(), N, M, N, K, _at(scratch), nbytes)
     return y
 
 

@@ -556,3 +556,35 @@ def test_quantised_block_as_it_is_used(dev):
     full = torch.relu((norm64(x, wn, r, 1e-6)[2]) @ w.double().t().contiguous()) + h.double()
     # each factor is off by at most 2^-4 of itself, in effect independently: 2^-4 / sqrt 3 each, together below 2^-4
     assert float((y.double() - full).norm() / (full - h.double()).norm()) < 2.0 ** -4
+
+
+# products that are cut along their reduction (few tiles, long sums) and whose unaligned operands are copied first
+@pytest.mark.parametrize("size", [(73, 409, 1280, 16), (73, 100, 3000, 0), (700, 520, 1021, 0), (1100, 515, 331, 129), (90, 1000, 5, 0),
+                                  (65, 64, 4096, 0), (520, 801, 63, 400), (200, 3, 2000, 0), (66, 2000, 17, 0)],
+                         ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_cut_and_copied(dev, dtype, size):
+    m, n, k, k2 = size
+    dt = TYPES[dtype]
+    for j, act in enumerate(("gelu", "none")):
+        x, w, b, r, g = make(dev, dt, m, n, k, k2, True, True, 500 + j, grad=True)
+        y = layers.linear(x[0] if k2 == 0 else tuple(x), w, b, act, r)
+        ref = Layer(x, w, b, r, act)
+        check(y.detach(), ref.y, ref.ey, "y")
+        gy = torch.randn(m, n, device=dev, generator=g).to(dt)
+        got = list(torch.autograd.grad(y, x + [w, b], gy))
+        (dx, ex), (dw, ew), (db, eb) = ref.gradients(gy)
+        check(torch.cat(got[:len(x)], -1), dx, ex, "dx")
+        check(got[len(x)], dw, ew, "dw")
+        check(got[len(x) + 1], db, eb, "db")
+
+
+def test_linear_q8_cut_and_copied(dev):
+    for m, n, k in ((73, 100, 3000), (700, 520, 1021), (128, 64, 4096)):
+        xq, xs, wq, ws, g = q8_operands(dev, m, n, k, 600 + m)
+        X, W = xq.double(), wq.double()
+        z = X @ W.t().contiguous() * xs.double()[:, None] * ws.double()
+        ez = (k + 6) * E * (X.abs() @ W.abs().t().contiguous()) * xs.double()[:, None] * ws.double()
+        check(layers.linear_q8(xq, xs, wq, ws, out_dtype=torch.float32), z, ez + E * z.abs(), "float32")
+        ez = ez + group_cut(X, W) * xs.double()[:, None] * ws.double()
+        check(layers.linear_q8(xq, xs, wq, ws), z, ez + half_step(torch.bfloat16) * (z.abs() + ez), "bf16")
