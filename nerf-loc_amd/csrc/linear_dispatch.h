@@ -22,19 +22,32 @@ inline bool dma_ok(int layout, const GemmArgs& g) {
     return true;
 }
 
+// The tile.  256 x 256 reads its operands least often and pays once every compute unit has one and sixteen k-tiles to work
+// through; 256 x 128 the same with half the outputs; below, and for short reductions, where filling and draining the
+// pipeline is the time, 128 x 64 runs three workgroups a unit beside each other, and 64 x 64 spreads what little there is.
+// Measured (us; 256 x 256, 256 x 128, 128 x 128, 128 x 64, 64 x 64):
+//   bf16 8192 x 4096 x 4096    258  295  318    -  444      bf16 4096 x 2048 x 2048   61  42  48  53  61
+//   bf16 4096 x 1024 x 4096    110   70   61   53   62      fp32 65536 x 256 x 320   111 107 108  98 101
+//   fp32 4096 x 4096 x 4096    994 1033 1098 1066 1099      8-bit 32768 x 1024 x 1024  83 75 66  65  74
 template <int DT, int LAY>
 int gemm_tiles(GemmArgs& g, hipStream_t s) {
-    auto tiles = [&](int n) { return ((g.P + n - 1) / n) * ((g.Q + n - 1) / n) * g.splits; };
-    if (dma_ok<DT>(LAY, g)) {
-        if constexpr (LAY != DW && elem_size(DT) == 2) {
-            if (g.nseg == 1 && !g.partial && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (g.Q <= 128 || g.seg[0].red <= 128 ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
-        }
-        if (LAY == FWD && DT != F8W && tiles(256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, DMA16>(g, s);
-        if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, DMA16>(g, s);
-        return launch<DT, LAY, 64, 64, 2, 2, DMA16>(g, s);
+    auto tiles = [&](int p, int q) { return ((g.P + p - 1) / p) * ((g.Q + q - 1) / q) * g.splits; };
+    if (!dma_ok<DT>(LAY, g)) {
+        if (tiles(128, 128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, REGS>(g, s);
+        return launch<DT, LAY, 64, 64, 2, 2, REGS>(g, s);
     }
-    if (tiles(128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, REGS>(g, s);
-    return launch<DT, LAY, 64, 64, 2, 2, REGS>(g, s);
+    if constexpr (LAY != DW && elem_size(DT) == 2) {
+        const bool narrow = g.Q <= 128 || g.seg[0].red <= 128;
+        if (g.nseg == 1 && !g.partial && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (narrow ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
+    }
+    const long long red = g.splits > 1 ? g.red_part : g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0);
+    const bool deep = red * elem_size(DT) >= 16 * 128;
+    if constexpr (LAY == FWD && DT != F8W) {       // the reduction-major layouts and the widened operands do not fit its registers
+        if (deep && tiles(256, 256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, DMA16>(g, s);
+    }
+    if (deep && tiles(256, 128) >= 256) return launch<DT, LAY, 256, 128, 4, 2, DMA16>(g, s);
+    if (tiles(128, 64) >= 400) return launch<DT, LAY, 128, 64, 2, 2, DMA16>(g, s);
+    return launch<DT, LAY, 64, 64, 2, 2, DMA16>(g, s);
 }
 
 template <int DT>
