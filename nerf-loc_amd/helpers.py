@@ -31,6 +31,19 @@ def get_default_precision():
     return _DEFAULT_PRECISION[0]
 
 
+# How NeRF evaluates networks that the fused kernels do not cover: None = library GEMMs layer by layer, else the package's
+# own layer operators (layers.py) on operands of this type; 'q8' holds the trunk's in 8 bits (inference, residual trunks)
+LAYER_PRECISIONS = (None, "fp32", "bf16", "fp16", "q8")
+_LAYER_PRECISION = [None]
+
+
+def set_layer_precision(name):
+    """The layer_precision of networks that do not set their own (see NeRF)."""
+    if name not in LAYER_PRECISIONS:
+        raise ValueError("unknown layer precision %r" % (name,))
+    _LAYER_PRECISION[0] = name
+
+
 # ---------------------------------------------------------------------------- positional encoding
 class Embedder:
     """Same keyword interface as run_nerf_helpers.py:15-45.  Only the
@@ -89,9 +102,20 @@ class NeRF(nn.Module):
     forward pass runs the fused MFMA kernel for the architecture the
     reference's configs use (D=8, W=256, skips=[4], input_ch=63,
     input_ch_views=27 with view directions, output_ch 4 or 5); other shapes
-    (--netdepth, --netwidth) are evaluated layer by layer with library GEMMs."""
+    (--netdepth, --netwidth) are evaluated layer by layer, with library GEMMs or,
+    with ``layer_precision`` (or set_layer_precision) 'fp32', 'bf16' or 'fp16',
+    with this package's layer operators: one launch per layer with bias, ReLU and
+    skip connection inside, float32 sums, float32 parameters and results.
 
-    def __init__(self, D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4], use_viewdirs=False):
+    residual=True (not in the reference) makes layers 1 .. D-1 of the trunk
+    residual blocks h <- h + relu(W_i norm(h) + b_i) with a root-mean-square norm
+    (weights ``norm_weights.i``), for trunks much deeper than eight layers.  They
+    run on the layer operators (float32 unless layer_precision says otherwise);
+    layer_precision 'q8' then holds the blocks' operands in 8 bits with a scale a
+    row (inference only; everything else in bf16)."""
+
+    def __init__(self, D=8, W=256, input_ch=3, input_ch_views=3, output_ch=4, skips=[4], use_viewdirs=False,
+                 residual=False):
         super(NeRF, self).__init__()
         self.D = D
         self.W = W
@@ -102,6 +126,8 @@ class NeRF(nn.Module):
         self.output_ch = output_ch
         self.precision = None          # None: follow set_default_precision()
         self.train_precision = None    # None: follow train.set_train_precision() (float32 unless changed)
+        self.layer_precision = None    # None: follow set_layer_precision()
+        self.residual = bool(residual)
         self._pack_cache = {}
 
         layers = [nn.Linear(input_ch, W)]
@@ -115,9 +141,13 @@ class NeRF(nn.Module):
             self.rgb_linear = nn.Linear(W // 2, 3)
         else:
             self.output_linear = nn.Linear(W, output_ch)
+        if self.residual:
+            self.norm_weights = nn.ParameterList([nn.Parameter(torch.ones(W)) for _ in range(D - 1)])
 
     # -- what the kernel can run
     def hip_supported(self):
+        if self.residual:
+            return False
         ok = (self.D == 8 and self.W == 256 and list(self.skips) == [4] and self.input_ch == 63)
         if self.use_viewdirs:
             return ok and self.input_ch_views == 27
@@ -132,8 +162,9 @@ class NeRF(nn.Module):
             raise NotImplementedError(
                 "NeRF: the HIP kernel implements D=8, W=256, skips=[4], input_ch=63 and input_ch_views=27 "
                 "(view directions) or output_ch in (4, 5) (no view directions); got D=%d W=%d skips=%s "
-                "input_ch=%d input_ch_views=%d output_ch=%d" % (self.D, self.W, list(self.skips), self.input_ch,
-                                                             self.input_ch_views, self.output_ch))
+                "input_ch=%d input_ch_views=%d output_ch=%d%s" % (self.D, self.W, list(self.skips), self.input_ch,
+                                                               self.input_ch_views, self.output_ch,
+                                                               " residual=True" if self.residual else ""))
 
     def precision_code(self):
         return hip.PRECISIONS[self.precision or get_default_precision()]
@@ -164,6 +195,10 @@ class NeRF(nn.Module):
         self._pack_cache[prec] = (key, packed)
         return packed
 
+    def __getstate__(self):
+        """Copies and pickles leave the packed and cast weights behind: they belong to this object's parameters."""
+        return dict(self.__dict__, _pack_cache={})
+
     def weights_changed(self):
         """Drops the packed copies.  Only needed after writes that bypass the version counters the cache is keyed on
         (`p.data.mul_(...)`, raw-pointer writes of foreign code); optimizers, `load_state_dict` and `copy_` are seen."""
@@ -190,10 +225,98 @@ class NeRF(nn.Module):
             h = F.relu(lin(h))
         return torch.cat([self.rgb_linear(h), alpha], -1)
 
+    # -- the layer operators
+    def _layer_tensors(self, prec, dt, grad):
+        """The layers' parameters as the operators take them: {layer: (weight, bias)} of type dt, norms as a list, and for
+        'q8' the blocks' weights in 8 bits.  With gradients, or while a graph is captured, cast by this call; otherwise
+        kept until a parameter changes, like packed_weights."""
+        from . import layers
+        params = list(self.parameters())
+        dev = params[0].device
+        keep = not grad and not torch.cuda.is_current_stream_capturing()
+        cur = torch.cuda.current_stream(dev)
+        if keep:
+            key = (hip.WEIGHT_GENERATION[0],) + tuple((p.data_ptr(), p._version) for p in params)
+            hit = self._pack_cache.get(("layers", prec))
+            if hit is not None and hit[0] == key:
+                if cur != hit[2]:              # made on another stream: behind its work, and not freed under this one's
+                    cur.wait_event(hit[3])
+                    for t in hit[4]:
+                        t.record_stream(cur)
+                return hit[1]
+        with torch.set_grad_enabled(grad):
+            cast = lambda p: p.to(dt) if grad else p.detach().to(dt)
+            out = {name: (cast(m.weight), cast(m.bias)) for name, m in self.named_modules() if isinstance(m, nn.Linear)}
+            out["norms"] = [cast(p) for p in self.norm_weights] if self.residual else []
+            if prec == "q8":
+                for i, lin in enumerate(self.pts_linears):
+                    if i > 0 and i - 1 not in self.skips:
+                        out["q8.%d" % i] = layers.quantize_weight(lin.weight)
+        if keep:
+            ev = torch.cuda.Event()
+            ev.record(cur)
+            flat = [t for v in out.values() for t in v]
+            self._pack_cache[("layers", prec)] = (key, out, cur, ev, flat)
+        return out
+
+    def _forward_layers(self, x, prec):
+        """The layers of run_nerf_helpers.py:96-119 (with residual, the blocks of the class's docstring) on the layer
+        operators: the ReLU, the bias, the skip connection and the residual are part of the launches."""
+        from . import layers
+        if not x.is_cuda:
+            raise ValueError("NeRF.forward: the input is on %s; this package computes on GPUs only" % x.device)
+        ch = self.input_ch + (self.input_ch_views if self.use_viewdirs else 0)
+        if x.shape[-1] < ch:
+            raise ValueError("NeRF.forward expects %d input channels, got %d" % (ch, x.shape[-1]))
+        grad = torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters()))
+        if prec == "q8" and not self.residual:
+            raise NotImplementedError("layer_precision 'q8' quantises the norms of a residual trunk (residual=True)")
+        if prec == "q8" and grad:
+            raise NotImplementedError("layer_precision 'q8' is for inference: train in 'fp32', 'bf16' or 'fp16', or call "
+                                      "under torch.no_grad()")
+        dt = {"fp32": torch.float32, "fp16": torch.float16}.get(prec, torch.bfloat16)
+        t = self._layer_tensors(prec, dt, grad)
+        with torch.cuda.device(x.device):
+            flat = x.reshape(-1, x.shape[-1])[:, :ch].to(dt)
+            pts = flat[:, :self.input_ch]
+            h = layers.linear(pts, *t["pts_linears.0"], activation="relu")
+            for i in range(1, self.D):
+                skip = i - 1 in self.skips
+                if not self.residual:
+                    h = layers.linear((pts, h) if skip else h, *t["pts_linears.%d" % i], activation="relu")
+                    continue
+                # the block's sum h + u is formed by the next block's norm, the last one's by its own epilogue
+                stream, u = (None, h) if i == 1 else (h, u)
+                last = i == self.D - 1
+                if prec == "q8" and not skip:
+                    q, s, h = layers.add_rms_norm_q8(u, t["norms"][i - 1], stream)
+                    u = layers.linear_q8(q, s, *t["q8.%d" % i], t["pts_linears.%d" % i][1], "relu", h if last else None, dt)
+                else:
+                    n, h = layers.add_rms_norm(u, t["norms"][i - 1], stream)
+                    u = layers.linear((pts, n) if skip else n, *t["pts_linears.%d" % i], activation="relu",
+                                      residual=h if last else None)
+                if last:
+                    h = u
+            if self.D - 1 in self.skips:
+                h = torch.cat([pts, h], -1)
+            if not self.use_viewdirs:
+                out = layers.linear(h, *t["output_linear"]).float()
+            else:
+                alpha = layers.linear(h, *t["alpha_linear"])
+                f = layers.linear(h, *t["feature_linear"])
+                f = layers.linear((f, flat[:, self.input_ch:]), *t["views_linears.0"], activation="relu")
+                out = torch.cat([layers.linear(f, *t["rgb_linear"]), alpha], -1).float()
+        return out.reshape(tuple(x.shape[:-1]) + (out.shape[-1],))
+
     def forward(self, x):
         """x: [..., input_ch + input_ch_views] encoded features -> [..., 4|output_ch]
         (run_nerf_helpers.py:96-119)."""
         if not self.hip_supported():
+            prec = self.layer_precision or _LAYER_PRECISION[0]
+            if prec not in LAYER_PRECISIONS:
+                raise ValueError("unknown layer precision %r" % (prec,))
+            if prec is not None or self.residual:
+                return self._forward_layers(x, prec or "fp32")
             return self._forward_library_gemms(x)
         ch = self.input_ch + (self.input_ch_views if self.use_viewdirs else 0)
         if x.shape[-1] < ch:
@@ -213,6 +336,8 @@ class NeRF(nn.Module):
         """Imports the weight list of the original TensorFlow release
         (run_nerf_helpers.py:121-148): kernels are stored [in, out] there."""
         assert self.use_viewdirs, "Not implemented if use_viewdirs=False"
+        if self.residual:
+            raise NotImplementedError("load_weights_from_keras: the TensorFlow release has no residual networks")
         def put(lin, k):
             lin.weight.data = torch.from_numpy(np.transpose(weights[k])).to(lin.weight.device)
             lin.bias.data = torch.from_numpy(np.transpose(weights[k + 1])).to(lin.bias.device)

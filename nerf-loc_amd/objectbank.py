@@ -77,7 +77,7 @@ class ObjectBank:
         if self.device.type != 'cuda':
             raise ValueError("ObjectBank keeps networks on a GPU; the template network is on %s" % self.device)
         self._ctor = dict(D=net.D, W=net.W, input_ch=net.input_ch, input_ch_views=net.input_ch_views,
-                          output_ch=net.output_ch, skips=list(net.skips), use_viewdirs=net.use_viewdirs)
+                          output_ch=net.output_ch, skips=list(net.skips), use_viewdirs=net.use_viewdirs, residual=net.residual)
         self._precision = precision if precision is not None else net.precision
         self.layout, self.total = state_dict_layout(net)
         self.capacity = capacity

@@ -16,7 +16,7 @@ import numpy as np
 import torch
 
 from . import hip
-from .helpers import NeRF, EmbedFn, get_embedder, to8b, _pdf_variates
+from .helpers import LAYER_PRECISIONS, NeRF, EmbedFn, get_embedder, to8b, _pdf_variates
 
 DEBUG = False
 
@@ -408,13 +408,20 @@ def create_nerf(args, device=None):
         embeddirs_fn, input_ch_views = get_embedder(args.multires_views, args.i_embed)
     output_ch = 5 if args.N_importance > 0 else 4
     skips = [4]
+    # not reference options: args.netresidual builds residual trunks, args.layer_precision selects how networks outside
+    # the fused kernels' shape are evaluated (see helpers.NeRF)
+    residual = bool(getattr(args, 'netresidual', False))
+    layer_precision = getattr(args, 'layer_precision', None)
+    if layer_precision not in LAYER_PRECISIONS:
+        raise ValueError("layer_precision must be one of %s, got %r" % (LAYER_PRECISIONS, layer_precision))
     model = NeRF(D=args.netdepth, W=args.netwidth, input_ch=input_ch, output_ch=output_ch, skips=skips,
-                 input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs).to(device)
+                 input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs, residual=residual).to(device)
     grad_vars = list(model.parameters())
     model_fine = None
     if args.N_importance > 0:
         model_fine = NeRF(D=args.netdepth_fine, W=args.netwidth_fine, input_ch=input_ch, output_ch=output_ch,
-                          skips=skips, input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs).to(device)
+                          skips=skips, input_ch_views=input_ch_views, use_viewdirs=args.use_viewdirs,
+                          residual=residual).to(device)
         grad_vars += list(model_fine.parameters())
     # not a reference option: args.train_precision = "bf16" trains with bf16 MFMA operands (float32 otherwise)
     train_precision = getattr(args, 'train_precision', None)
@@ -423,6 +430,8 @@ def create_nerf(args, device=None):
     for m in (model, model_fine):
         if m is not None and train_precision is not None:
             m.train_precision = train_precision
+        if m is not None:
+            m.layer_precision = layer_precision
     network_query_fn = NetworkQuery(embed_fn, embeddirs_fn, args.netchunk)
     from .train import FusedAdam      # torch.optim.Adam's update and state layout, one launch per step
     optimizer = FusedAdam(params=grad_vars, lr=args.lrate, betas=(0.9, 0.999))

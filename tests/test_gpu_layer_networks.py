@@ -1,0 +1,232 @@
+"""Networks outside the fused kernels' shape on the layer operators: forward against a 64-bit restatement, gradients against
+autograd on it, rendering and training through the package's own paths."""
+import copy
+import types
+
+import numpy as np
+import pytest
+import torch
+
+from nerf_loc_amd import helpers, layers, render, synth, train
+
+pytestmark = pytest.mark.gpu
+E = 2.0 ** -24
+
+
+@pytest.fixture(scope="module")
+def dev():
+    return torch.device("cuda:0")
+
+
+def net64(net, x):
+    """The network in float64, written from its definition."""
+    P = {k: v.detach().double().requires_grad_(v.requires_grad) for k, v in net.named_parameters()}
+    lin = lambda name, h: h @ P[name + ".weight"].t() + P[name + ".bias"]
+    x = x.double()
+    pts = x[..., :net.input_ch]
+    h = torch.relu(lin("pts_linears.0", pts))
+    for i in range(1, net.D):
+        skip = (i - 1) in net.skips
+        if net.residual:
+            n = h / torch.sqrt((h * h).mean(-1, keepdim=True) + 1e-6) * P["norm_weights.%d" % (i - 1)]
+            h = h + torch.relu(lin("pts_linears.%d" % i, torch.cat([pts, n], -1) if skip else n))
+        else:
+            h = torch.relu(lin("pts_linears.%d" % i, torch.cat([pts, h], -1) if skip else h))
+    if not net.use_viewdirs:
+        return lin("output_linear", h), P
+    alpha = lin("alpha_linear", h)
+    f = torch.relu(lin("views_linears.0", torch.cat([lin("feature_linear", h), x[..., net.input_ch:net.input_ch + net.input_ch_views]], -1)))
+    return torch.cat([lin("rgb_linear", f), alpha], -1), P
+
+
+def build(dev, seed=0, **kw):
+    torch.manual_seed(seed)
+    args = dict(D=6, W=96, input_ch=63, output_ch=4, skips=[2], input_ch_views=27, use_viewdirs=True)
+    args.update(kw)
+    net = helpers.NeRF(**args).to(dev)
+    if net.residual:
+        with torch.no_grad():
+            for p in net.norm_weights:
+                p.uniform_(0.5, 1.5)
+    return net
+
+
+SHAPES = [dict(), dict(use_viewdirs=False, output_ch=5), dict(D=4, W=128, skips=[]), dict(residual=True),
+          dict(residual=True, D=12, W=64, skips=[4, 8]), dict(residual=True, D=2, W=40, skips=[], use_viewdirs=False), dict(D=1, W=48, skips=[])]
+
+
+@pytest.mark.parametrize("shape", SHAPES, ids=str)
+def test_forward_and_gradients(dev, shape):
+    net = build(dev, **shape)
+    net.layer_precision = "fp32"
+    x = torch.rand(7, 50, 90, device=dev) * 2 - 1
+    with torch.no_grad():
+        y = net(x)
+    want, P = net64(net, x)
+    assert y.dtype == torch.float32 and tuple(y.shape) == tuple(want.shape)
+    # forward error analysis, layer by layer, gives depth * (width + a few) * e relative to the magnitudes that meet; these
+    # networks' values are of order one, and 2e-5 is that bound for depth 13 and width 130 with factor 12 to spare
+    assert float((y.double() - want).abs().max()) < 2e-5 * max(1.0, float(want.detach().abs().max()))
+    g = torch.randn(want.shape, device=dev)
+    y = net(x)
+    y.backward(g)
+    (want * g.double()).sum().backward()
+    for k, p in net.named_parameters():
+        if P[k].grad is None:
+            assert p.grad is None, k
+            continue
+        # relu signs of arguments within float32 rounding of zero may differ: their share of a sum of 350 samples' gradients
+        scale = float(P[k].grad.norm()) + 1e-12
+        assert float((p.grad.double() - P[k].grad).norm()) < 1e-3 * scale, k
+
+
+@pytest.mark.parametrize("prec", ["bf16", "fp16", "q8"])
+def test_lower_precisions_stay_near(dev, prec):
+    """Roundings of operands: 2^-9, 2^-12, or about 2^-5 (8 bits) relative per layer, adding up as independent over the
+    eleven matrix products in a row; factor four on that."""
+    net = build(dev, residual=True, D=8, W=128, skips=[3])
+    net.layer_precision = prec
+    x = torch.rand(400, 90, device=dev) * 2 - 1
+    with torch.no_grad():
+        y = net(x)
+        net.layer_precision = "fp32"
+        ref = net(x)
+    u = {"bf16": 2.0 ** -9, "fp16": 2.0 ** -12, "q8": 2.0 ** -5}[prec]
+    assert y.dtype == torch.float32
+    assert float((y - ref).norm() / ref.norm()) < 4 * u * 11 ** 0.5
+    assert float((y - ref).abs().max()) > 0
+
+
+def test_default_path_is_untouched(dev):
+    """Without layer_precision other shapes run as they did (library GEMMs): same bits with and without the new setting's
+    default, double backward included."""
+    net = build(dev)
+    x = (torch.rand(30, 90, device=dev) * 2 - 1).requires_grad_()
+    y = net(x)
+    assert torch.equal(y, net._forward_library_gemms(x))
+    gx, = torch.autograd.grad(y[:, 3].sum(), x, create_graph=True)
+    gx.square().sum().backward()
+    assert net.pts_linears[0].weight.grad is not None
+
+
+def test_global_setting_and_refusals(dev):
+    net = build(dev)
+    x = torch.rand(30, 90, device=dev)
+    try:
+        helpers.set_layer_precision("bf16")
+        with torch.no_grad():
+            a = net(x)
+            net.layer_precision = "bf16"
+            assert torch.equal(a, net(x))
+    finally:
+        helpers.set_layer_precision(None)
+    with pytest.raises(ValueError):
+        helpers.set_layer_precision("int4")
+    net.layer_precision = "q8"
+    with pytest.raises(NotImplementedError, match="residual"):
+        net(x)
+    res = build(dev, residual=True)
+    res.layer_precision = "q8"
+    with pytest.raises(NotImplementedError, match="inference"):
+        res(x)
+    with pytest.raises(ValueError, match="input channels"):
+        res(x[:, :50])
+    with pytest.raises(ValueError, match="GPUs only"):
+        res(x.cpu())
+    with pytest.raises(NotImplementedError, match="residual"):
+        res.packed_weights()
+
+
+def test_cast_weights_follow_the_parameters(dev):
+    """In-place changes, FusedAdam's raw writes, and a second stream."""
+    net = build(dev, residual=True)
+    net.layer_precision = "bf16"
+    x = torch.rand(64, 90, device=dev)
+    with torch.no_grad():
+        a = net(x)
+        net.pts_linears[1].weight.mul_(0.5)
+        b = net(x)
+    assert not torch.equal(a, b)
+    opt = train.FusedAdam(net.parameters(), lr=1e-2)
+    net(x).square().sum().backward()
+    opt.step()
+    with torch.no_grad():
+        c = net(x)
+        assert not torch.equal(b, c)
+        net.weights_changed()
+        assert torch.equal(net(x), c)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            d = net(x)
+        torch.cuda.current_stream().wait_stream(side)
+        assert torch.equal(c, d)
+
+
+def test_graph_capture_of_a_residual_network(dev):
+    for prec in ("bf16", "q8"):
+        net = build(dev, residual=True)
+        net.layer_precision = prec
+        x = torch.rand(300, 90, device=dev)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.no_grad():
+            with torch.cuda.stream(side):
+                net(x)
+            torch.cuda.current_stream().wait_stream(side)
+            graph = torch.cuda.CUDAGraph()
+            with torch.cuda.graph(graph):
+                y = net(x)
+            for k in range(3):
+                x.uniform_(-1, 1)
+                net.pts_linears[2].weight.mul_(0.9)
+                y.zero_()
+                graph.replay()
+                torch.cuda.synchronize()
+                assert torch.equal(y, net(x)), (prec, k)
+
+
+def test_render_and_train_through_the_package(dev):
+    """create_nerf with a residual trunk: a render in three precisions, training steps, a checkpoint round trip."""
+    import tempfile
+    with tempfile.TemporaryDirectory() as tmp:
+        args = types.SimpleNamespace(multires=10, i_embed=0, use_viewdirs=True, multires_views=4, N_importance=16, netdepth=6,
+                                     netwidth=64, netdepth_fine=6, netwidth_fine=64, netchunk=65536, lrate=5e-4, basedir=tmp,
+                                     expname="x", ft_path=None, no_reload=True, perturb=0., N_samples=16, white_bkgd=True,
+                                     raw_noise_std=0., dataset_type="blender", no_ndc=True, lindisp=False, netresidual=True,
+                                     layer_precision="fp32")
+        torch.manual_seed(3)
+        kw_train, kw_test, _, params, opt = render.create_nerf(args, dev)
+        assert kw_train["network_fn"].residual and not kw_train["network_fn"].hip_supported()
+        rays = torch.from_numpy(synth.random_rays(64, seed=4)).to(dev)
+        target = torch.rand(64, 3, device=dev)
+        losses = [float(train.train_step(rays, target, kw_train, opt, k, 5e-4, 250)[0]) for k in range(3)]
+        assert all(np.isfinite(losses)) and any(p.grad is not None and float(p.grad.abs().max()) > 0 for p in params)
+        render_kw = {k: v for k, v in kw_test.items() if k not in ("use_viewdirs", "ndc", "near", "far")}
+        with torch.no_grad():
+            a = render.render_rays(rays, **render_kw)["rgb_map"]
+            for prec in ("bf16", "q8"):
+                for n in ("network_fn", "network_fine"):
+                    kw_test[n].layer_precision = prec
+                b = render.render_rays(rays, **render_kw)["rgb_map"]
+                assert bool(torch.isfinite(b).all()) and float((a - b).abs().mean()) < 0.1
+            for n in ("network_fn", "network_fine"):
+                kw_test[n].layer_precision = "fp32"
+        path = tmp + "/c.tar"
+        render.save_checkpoint(path, 3, kw_train["network_fn"], kw_train["network_fine"], opt)
+        other = render.create_nerf(args, dev)[1]
+        render.load_checkpoint(path, other["network_fn"], other["network_fine"])
+        with torch.no_grad():
+            assert torch.equal(render.render_rays(rays, **{**render_kw, "network_fn": other["network_fn"],
+                                                           "network_fine": other["network_fine"]})["rgb_map"], a)
+
+
+def test_module_copies_and_state_dicts(dev):
+    net = build(dev, residual=True)
+    assert [k for k in net.state_dict() if k.startswith("norm_weights")] == ["norm_weights.%d" % i for i in range(5)]
+    x = torch.rand(9, 90, device=dev)
+    with torch.no_grad():
+        a = net(x)
+        twin = copy.deepcopy(net)
+        assert torch.equal(twin(x), a)
+    assert not any("norm" in k for k in build(dev).state_dict())
