@@ -50,7 +50,7 @@ struct GemmArgs {
     long long ldr, ldy, ldz;
     const float *sp, *sq;        // 8-bit operands: scales of the rows of A and of B
     int act;
-    int out_dt;                  // type of y, bias, res, z
+    int out_dt;                  // type of y, bias, res, z: the operands' own, or named by the call for 8-bit ones
     unsigned tiles_p, tiles_q;
 };
 
@@ -71,7 +71,7 @@ enum Layout { FWD = 0, DX = 1, DW = 2 };
 int gemm_f32(int layout, GemmArgs& g, hipStream_t s);
 int gemm_bf16(int layout, GemmArgs& g, hipStream_t s);
 int gemm_f16(int layout, GemmArgs& g, hipStream_t s);
-int gemm_f8(GemmArgs& g, hipStream_t s);
+int gemm_f8(GemmArgs& g, hipStream_t s);                 // out_dt names the epilogue's type
 // out [rows, cols] (rows ldo apart) = sum over n parts [rows][cols], in a fixed order (linear.hip)
 int part_sum(int dtype, const float* parts, int n, long long rows, long long cols, void* out, long long ldo, hipStream_t s);
 
@@ -171,57 +171,42 @@ __device__ __forceinline__ float act_grad(float z, int act) {
         default: return 1.f;
     }
 }
-// the epilogue's types: of the operands, or, for 8-bit operands, named by the call
-template <int DT>
-__device__ __forceinline__ void load8(const void* p, long long i, float (&v)[8], int dt) {
-    if constexpr (!is_f8(DT)) ld8<DT>(p, i, v);
-    else if (dt == F32) ld8<F32>(p, i, v);
-    else if (dt == BF16) ld8<BF16>(p, i, v);
-    else ld8<F16>(p, i, v);
-}
-template <int DT>
-__device__ __forceinline__ void store8(void* p, long long i, const float (&v)[8], int dt) {
-    if constexpr (!is_f8(DT)) st8<DT>(p, i, v);
-    else if (dt == F32) st8<F32>(p, i, v);
-    else if (dt == BF16) st8<BF16>(p, i, v);
-    else st8<F16>(p, i, v);
-}
-
 // Eight columns of one row.  Both ways out (a whole group by 16-byte accesses, the last columns one by one) share the
 // arithmetic in between.
 template <int DT>
-__device__ __forceinline__ void some8(const void* p, long long i, bool whole, int n, float (&v)[8], int dt) {
-    if (whole) load8<DT>(p, i, v, dt);
+__device__ __forceinline__ void some8(const void* p, long long i, bool whole, int n, float (&v)[8]) {
+    if (whole) ld8<DT>(p, i, v);
     else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) v[j] = j < n ? ld_elem(p, i + j, is_f8(DT) ? dt : DT) : 0.f;
+        for (int j = 0; j < 8; ++j) v[j] = j < n ? ld_elem(p, i + j, DT) : 0.f;
     }
 }
 template <int DT>
-__device__ __forceinline__ void put_some8(void* p, long long i, bool whole, int n, const float (&v)[8], int dt) {
-    if (whole) store8<DT>(p, i, v, dt);
+__device__ __forceinline__ void put_some8(void* p, long long i, bool whole, int n, const float (&v)[8]) {
+    if (whole) st8<DT>(p, i, v);
     else {
 #pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) st_elem(p, i + j, v[j], is_f8(DT) ? dt : DT);
+        for (int j = 0; j < 8; ++j) if (j < n) st_elem(p, i + j, v[j], DT);
     }
 }
-template <int DT>
+// DT: type of bias, residual, z and y.  SCALED: sums of 8-bit operands, to be scaled by row and column first.
+template <int DT, bool SCALED>
 __device__ __forceinline__ void epilogue8(const GemmArgs& g, long long p, long long q, float (&v)[8]) {
     const bool whole = q + 8 <= g.Q;
     const int n = whole ? 8 : (int)(g.Q - q);
     float t[8];
-    if constexpr (is_f8(DT)) {
+    if constexpr (SCALED) {
         const float s = g.sp[p];
-        some8<F32>(g.sq, q, whole, n, t, F32);
+        some8<F32>(g.sq, q, whole, n, t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = v[j] * s * t[j];
     }
     if (g.bias) {
-        some8<DT>(g.bias, q, whole, n, t, g.out_dt);
+        some8<DT>(g.bias, q, whole, n, t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += t[j];
     }
-    if (g.z) put_some8<DT>(g.z, p * g.ldz + q, whole, n, v, g.out_dt);
+    if (g.z) put_some8<DT>(g.z, p * g.ldz + q, whole, n, v);
     if (g.act == NERF_ACT_RELU) {
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] = act_fn(v[j], NERF_ACT_RELU);
@@ -233,11 +218,11 @@ __device__ __forceinline__ void epilogue8(const GemmArgs& g, long long p, long l
         for (int j = 0; j < 8; ++j) v[j] = act_fn(v[j], NERF_ACT_SILU);
     }
     if (g.res) {
-        some8<DT>(g.res, p * g.ldr + q, whole, n, t, g.out_dt);
+        some8<DT>(g.res, p * g.ldr + q, whole, n, t);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += t[j];
     }
-    put_some8<DT>(g.y, p * g.ldy + q, whole, n, v, g.out_dt);
+    put_some8<DT>(g.y, p * g.ldy + q, whole, n, v);
 }
 
 // ---------------------------------------------------------------------------------------------- one operand's tile
@@ -497,8 +482,8 @@ struct Loader {
 template <int WP, int WQ>
 __host__ __device__ constexpr int epi_bytes() { return 16 * (WQ + 4) * 4; }
 
-// BP x BQ of C per workgroup of WVP x WVQ waves.
-template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
+// BP x BQ of C per workgroup of WVP x WVQ waves; ODT: the epilogue's type.
+template <int DT, int ODT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
 __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     constexpr int NT = WVP * WVQ * 64;
     constexpr int TA = LAY == DW, TB = LAY != FWD;
@@ -674,19 +659,19 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
 #pragma unroll
                         for (int j = 0; j < 8; ++j) if (q + j < g.Q) o[j] = v[j];
                     }
-                } else epilogue8<DT>(g, p, q, v);
+                } else epilogue8<ODT, is_f8(DT)>(g, p, q, v);
             }
         }
     }
 }
 
-template <int DT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
+template <int DT, int ODT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
 int launch(GemmArgs& g, hipStream_t s) {
     const long long tp = (g.P + BP - 1) / BP, tq = (g.Q + BQ - 1) / BQ;
     NERF_REQUIRE(tp * tq < (1ll << 31), "linear: %lld x %lld outputs are too many for one launch", g.P, g.Q);
     g.tiles_p = (unsigned)tp;
     g.tiles_q = (unsigned)tq;
-    auto k = gemm_kernel<DT, LAY, BP, BQ, WVP, WVQ, WAY>;
+    auto k = gemm_kernel<DT, ODT, LAY, BP, BQ, WVP, WVQ, WAY>;
     hipLaunchKernelGGL(k, dim3((unsigned)(tp * tq), g.splits), dim3(WVP * WVQ * 64), 0, s, g);
     NERF_LAUNCH_CHECK();
     return NERF_OK;
@@ -708,7 +693,7 @@ __device__ __forceinline__ i32x4 chunk_at(const char* p, long long have) {
     return v;
 }
 
-template <int DT, int MT, int NW>
+template <int DT, int ODT, int MT, int NW>
 __global__ void __launch_bounds__(NW * 64) few_rows_kernel(const GemmArgs g) {
     constexpr int E = elem_size(DT), CE = 16 / E, STEP = 4 * CE, U = (MT == 1 ? 8 : MT == 2 ? 4 : 2) / (DT == F8W ? 2 : 1);
     __shared__ __align__(16) float sums[NW][MT][16][20];
@@ -762,18 +747,18 @@ __global__ void __launch_bounds__(NW * 64) few_rows_kernel(const GemmArgs g) {
         for (int k = 0; k < NW; ++k)
 #pragma unroll
             for (int j = 0; j < 8; ++j) v[j] += sums[k][p >> 4][p & 15][col + j];
-        if (p < g.P && q0 + col < g.Q) epilogue8<DT>(g, p, q0 + col, v);
+        if (p < g.P && q0 + col < g.Q) epilogue8<ODT, is_f8(DT)>(g, p, q0 + col, v);
     }
 }
 
-template <int DT, int MT>
+template <int DT, int ODT, int MT>
 int launch_few_rows(GemmArgs& g, hipStream_t s) {
     const dim3 grid((unsigned)((g.Q + 15) / 16));
     // sixteen waves (eight where widening needs the registers) once each has two steps to take, else four
     constexpr int MANY = DT == F8W ? 8 : 16;
     const long long bytes = (g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0)) * elem_size(DT);
-    if (bytes >= 32 * 64) hipLaunchKernelGGL((few_rows_kernel<DT, MT, MANY>), grid, dim3(MANY * 64), 0, s, g);
-    else hipLaunchKernelGGL((few_rows_kernel<DT, MT, 4>), grid, dim3(256), 0, s, g);
+    if (bytes >= 32 * 64) hipLaunchKernelGGL((few_rows_kernel<DT, ODT, MT, MANY>), grid, dim3(MANY * 64), 0, s, g);
+    else hipLaunchKernelGGL((few_rows_kernel<DT, ODT, MT, 4>), grid, dim3(256), 0, s, g);
     NERF_LAUNCH_CHECK();
     return NERF_OK;
 }

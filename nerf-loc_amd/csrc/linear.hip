@@ -123,7 +123,7 @@ int part_sum(int dtype, const float* parts, int n, long long rows, long long col
 }
 
 // The epilogue on the sums of a split product: one thread adds eight columns' parts, in order.
-template <int DT>
+template <int DT, bool SCALED>
 __global__ void __launch_bounds__(256) finish_kernel(const GemmArgs g, int parts) {
     const long long groups = (g.Q + 7) / 8, t = (long long)blockIdx.x * 256 + threadIdx.x;
     const long long p = t / groups, q = t % groups * 8;
@@ -133,11 +133,11 @@ __global__ void __launch_bounds__(256) finish_kernel(const GemmArgs g, int parts
     float v[8] = {};
     for (int k = 0; k < parts; ++k) {
         float t8[8];
-        some8<F32>(g.partial, ((long long)k * g.P + p) * g.Q + q, whole, n, t8, F32);
+        some8<F32>(g.partial, ((long long)k * g.P + p) * g.Q + q, whole, n, t8);
 #pragma unroll
         for (int j = 0; j < 8; ++j) v[j] += t8[j];
     }
-    epilogue8<DT>(g, p, q, v);
+    epilogue8<DT, SCALED>(g, p, q, v);
 }
 
 // Rows copied to places on 16 bytes, zeros behind their ends to a whole chunk.  One chunk a thread.
@@ -255,11 +255,12 @@ struct Product {
         int rc = dispatch_gemm(dtype, layout, g, st);
         if (rc != NERF_OK) return rc;
         const dim3 grid((unsigned)((P * ((Q + 7) / 8) + 255) / 256));
-        switch (dtype) {
-            case F32: hipLaunchKernelGGL(finish_kernel<F32>, grid, dim3(256), 0, st, g, g.splits); break;
-            case BF16: hipLaunchKernelGGL(finish_kernel<BF16>, grid, dim3(256), 0, st, g, g.splits); break;
-            case F16: hipLaunchKernelGGL(finish_kernel<F16>, grid, dim3(256), 0, st, g, g.splits); break;
-            default: hipLaunchKernelGGL(finish_kernel<F8>, grid, dim3(256), 0, st, g, g.splits); break;
+        auto finish = [&](auto k) { hipLaunchKernelGGL(k, grid, dim3(256), 0, st, g, g.splits); };
+        const bool scaled = dtype == F8;
+        switch (g.out_dt) {
+            case F32: scaled ? finish(finish_kernel<F32, true>) : finish(finish_kernel<F32, false>); break;
+            case BF16: scaled ? finish(finish_kernel<BF16, true>) : finish(finish_kernel<BF16, false>); break;
+            default: scaled ? finish(finish_kernel<F16, true>) : finish(finish_kernel<F16, false>); break;
         }
         NERF_LAUNCH_CHECK();
         return NERF_OK;

@@ -29,12 +29,12 @@ inline bool dma_ok(int layout, const GemmArgs& g) {
 //   bf16 8192 x 4096 x 4096    258  295  318    -  444      bf16 4096 x 2048 x 2048   61  42  48  53  61
 //   bf16 4096 x 1024 x 4096    110   70   61   53   62      fp32 65536 x 256 x 320   111 107 108  98 101
 //   fp32 4096 x 4096 x 4096    994 1033 1098 1066 1099      8-bit 32768 x 1024 x 1024  83 75 66  65  74
-template <int DT, int LAY>
+template <int DT, int ODT, int LAY>
 int gemm_tiles(GemmArgs& g, hipStream_t s) {
     auto tiles = [&](int p, int q) { return ((g.P + p - 1) / p) * ((g.Q + q - 1) / q) * g.splits; };
     if (!dma_ok<DT>(LAY, g)) {
-        if (tiles(128, 128) >= 256) return launch<DT, LAY, 128, 128, 2, 2, REGS>(g, s);
-        return launch<DT, LAY, 64, 64, 2, 2, REGS>(g, s);
+        if (tiles(128, 128) >= 256) return launch<DT, ODT, LAY, 128, 128, 2, 2, REGS>(g, s);
+        return launch<DT, ODT, LAY, 64, 64, 2, 2, REGS>(g, s);
     }
     if constexpr (LAY != DW && elem_size(DT) == 2) {
         const bool narrow = g.Q <= 128 || g.seg[0].red <= 128;
@@ -43,27 +43,28 @@ int gemm_tiles(GemmArgs& g, hipStream_t s) {
     const long long red = g.splits > 1 ? g.red_part : g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0);
     const bool deep = red * elem_size(DT) >= 16 * 128;
     if constexpr (LAY == FWD && DT != F8W) {       // the reduction-major layouts and the widened operands do not fit its registers
-        if (deep && tiles(256, 256) >= 256) return launch<DT, LAY, 256, 256, 2, 4, DMA16>(g, s);
+        if (deep && tiles(256, 256) >= 256) return launch<DT, ODT, LAY, 256, 256, 2, 4, DMA16>(g, s);
     }
-    if (deep && tiles(256, 128) >= 256) return launch<DT, LAY, 256, 128, 4, 2, DMA16>(g, s);
-    if (tiles(128, 64) >= 400) return launch<DT, LAY, 128, 64, 2, 2, DMA16>(g, s);
-    return launch<DT, LAY, 64, 64, 2, 2, DMA16>(g, s);
+    if (deep && tiles(256, 128) >= 256) return launch<DT, ODT, LAY, 256, 128, 4, 2, DMA16>(g, s);
+    if (tiles(128, 64) >= 400) return launch<DT, ODT, LAY, 128, 64, 2, 2, DMA16>(g, s);
+    return launch<DT, ODT, LAY, 64, 64, 2, 2, DMA16>(g, s);
 }
 
-template <int DT>
+template <int DT, int ODT>
 int gemm_forward(GemmArgs& g, hipStream_t s) {
-    if (g.P <= 16) return launch_few_rows<DT == F8 ? F8W : DT, 1>(g, s);
-    if (g.P <= 32) return launch_few_rows<DT == F8 ? F8W : DT, 2>(g, s);
-    if (g.P <= FEW_ROWS) return launch_few_rows<DT == F8 ? F8W : DT, 4>(g, s);
-    return gemm_tiles<DT, FWD>(g, s);
+    constexpr int D = DT == F8 ? F8W : DT;       // few rows: widening is hidden behind the weights' loads
+    if (g.P <= 16) return launch_few_rows<D, ODT, 1>(g, s);
+    if (g.P <= 32) return launch_few_rows<D, ODT, 2>(g, s);
+    if (g.P <= FEW_ROWS) return launch_few_rows<D, ODT, 4>(g, s);
+    return gemm_tiles<DT, ODT, FWD>(g, s);
 }
 
 template <int DT>
 int gemm(int layout, GemmArgs& g, hipStream_t s) {
     switch (layout) {
-        case FWD: return gemm_forward<DT>(g, s);
-        case DX: return gemm_tiles<DT, DX>(g, s);
-        default: return gemm_tiles<DT, DW>(g, s);
+        case FWD: return gemm_forward<DT, DT>(g, s);
+        case DX: return gemm_tiles<DT, DT, DX>(g, s);
+        default: return gemm_tiles<DT, DT, DW>(g, s);
     }
 }
 

@@ -133,16 +133,24 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
             *reinterpret_cast<uint4*>(wlds + q * ROWB + ((c & ~7) | ((c ^ q) & 7)) * 16) = v;
         }
     } else {
-        // eight columns of one reduction row at a time, turned by single stores: 128 KB once per workgroup
-        for (int t = tid; t < H * NF * 2 * KS * 32; t += 512) {
-            const int r = t / (H * NF * 2), q0 = t % (H * NF * 2) * 8;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (r < K && q0 < Q) v = *reinterpret_cast<const uint4*>(static_cast<const char*>(g.seg[0].b) + ((long long)r * g.seg[0].ldb + q0) * 2);
-            const unsigned short* e = reinterpret_cast<const unsigned short*>(&v);
+        // 8 x 8 blocks turned in registers: eight reduction rows of eight columns in, eight chunks of a column's rows out
+        for (int t = tid; t < H * NF * 2 * KS * 4; t += 512) {
+            const int c = t / (H * NF * 2), q0 = t % (H * NF * 2) * 8;
+            unsigned in[8][4];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (c * 8 + r < K && q0 < Q) v = *reinterpret_cast<const uint4*>(static_cast<const char*>(g.seg[0].b) + ((long long)(c * 8 + r) * g.seg[0].ldb + q0) * 2);
+                in[r][0] = v.x; in[r][1] = v.y; in[r][2] = v.z; in[r][3] = v.w;
+            }
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                const int q = q0 + j, c = r >> 3;
-                *reinterpret_cast<unsigned short*>(wlds + q * ROWB + ((c & ~7) | ((c ^ q) & 7)) * 16 + (r & 7) * 2) = e[j];
+                const int q = q0 + j;
+                unsigned out[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k)
+                    out[k] = __builtin_amdgcn_perm(in[2 * k + 1][j >> 1], in[2 * k][j >> 1], j & 1 ? 0x07060302 : 0x05040100);
+                *reinterpret_cast<uint4*>(wlds + q * ROWB + ((c & ~7) | ((c ^ q) & 7)) * 16) = make_uint4(out[0], out[1], out[2], out[3]);
             }
         }
     }
@@ -150,6 +158,15 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
     __syncthreads();
 
     const unsigned char* wl = wlds + (half + i) * ROWB;
+    // a step's weight fragments are read while the step before it is worked on; the first step's are those of every block
+    i32x4 w[2][NF];
+    auto weights = [&](int s) {
+        const int place = ((4 * s & ~7) | (((4 * s + gr) & 7) ^ (i & 7))) * 16;
+#pragma unroll
+        for (int j = 0; j < NF; ++j) w[s & 1][j] = *reinterpret_cast<const i32x4*>(wl + j * 16 * ROWB + place);
+    };
+    static_assert(KS % 2 == 0, "the first step's fragments follow the last one's");
+    weights(0);
     for (; blk < blocks; blk += stride) {
         const bool more = blk + stride < blocks;
         if (more) aim(blk + stride);
@@ -162,14 +179,12 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
         }
 #pragma unroll
         for (int s = 0; s < KS; ++s) {
-            const int place = ((4 * s & ~7) | ((4 * s + gr) & 7 ^ i & 7)) * 16;
+            weights((s + 1) % KS);
+            __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-            for (int j = 0; j < NF; ++j) {
-                const i32x4 w = *reinterpret_cast<const i32x4*>(wl + j * 16 * ROWB + place);
+            for (int j = 0; j < NF; ++j)
 #pragma unroll
-                for (int r = 0; r < RF; ++r) mma<DT>(acc[r][j], w, __builtin_bit_cast(i32x4, x[r][s]));
-                if (j % 8 == 7) __builtin_amdgcn_sched_barrier(0);       // eight weight fragments at a time: registers
-            }
+                for (int r = 0; r < RF; ++r) mma<DT>(acc[r][j], w[s & 1][j], __builtin_bit_cast(i32x4, x[r][s]));
             if (more) fetch(s);
             __builtin_amdgcn_sched_barrier(0);
         }

@@ -52,6 +52,39 @@ __device__ __forceinline__ void put8(void* p, long long base, int c, int n, cons
     }
 }
 
+// Eight elements as they lie in memory.
+template <int DT>
+struct Raw {
+    static constexpr int E = elem_size(DT);
+    unsigned v[2 * E];
+    __device__ __forceinline__ void get(const void* p, long long base, int c, int n) {
+        const char* q = static_cast<const char*>(p) + (base + c) * E;
+        if (c + 8 <= n) __builtin_memcpy(v, q, 8 * E);
+        else {
+#pragma unroll
+            for (int j = 0; j < 2 * E; ++j) v[j] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                if (c + j < n) {
+                    if constexpr (E == 4) v[j] = reinterpret_cast<const unsigned*>(q)[j];
+                    else v[j >> 1] |= (unsigned)reinterpret_cast<const unsigned short*>(q)[j] << (16 * (j & 1));
+                }
+            }
+        }
+    }
+    __device__ __forceinline__ void put(float (&f)[8]) const {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) {
+            if constexpr (DT == F32) f[j] = __uint_as_float(v[j]);
+            else if constexpr (DT == BF16) f[j] = __uint_as_float(j & 1 ? v[j >> 1] & 0xffff0000u : v[j >> 1] << 16);
+            else {
+                const unsigned short u = (unsigned short)(v[j >> 1] >> (16 * (j & 1)));
+                f[j] = (float)__builtin_bit_cast(_Float16, u);
+            }
+        }
+    }
+};
+
 // Sum (or, of absolute values' bits, the maximum: NaN above infinity above all numbers) over the ROWT threads of a row.
 template <int ROWT>
 __device__ __forceinline__ float row_sum(float v, float* shared) {
@@ -179,20 +212,28 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_grad_kernel(cons
         const bool live = row < a.M;
         const long long rw = live ? row : a.M - 1;
         const float rstd = a.rstd[rw];
-        float h[VPT][8], n[VPT][8], dot = 0.f;
+        // everything the row needs is asked for at once, and stays as it came (packed, for 16-bit types) until used
+        Raw<DT> h[VPT], gy[VPT], gh[VPT], w[VPT];
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int c = (k * ROWT + t) * 8;
-            float w[8], gy[8];
-            row8<DT>(a.h, rw * a.ldh, c, a.N, h[k]);
-            row8<DT>(a.w, 0, c, a.N, w);
-            row8<DT>(a.gy, rw * a.ldgy, c, a.N, gy);
+            h[k].get(a.h, rw * a.ldh, c, a.N);
+            gy[k].get(a.gy, rw * a.ldgy, c, a.N);
+            if (a.gh) gh[k].get(a.gh, rw * a.ldgh, c, a.N);
+            w[k].get(a.w, 0, c, a.N);
+        }
+        float dot = 0.f;
+#pragma unroll
+        for (int k = 0; k < VPT; ++k) {
+            float hv[8], gv[8], wv[8];
+            h[k].put(hv);
+            gy[k].put(gv);
+            w[k].put(wv);
 #pragma unroll
             for (int j = 0; j < 8; ++j) {
-                h[k][j] *= rstd;
-                if (live) dw[k][j] = fmaf(gy[j], h[k][j], dw[k][j]);
-                n[k][j] = gy[j] * w[j];
-                dot = fmaf(n[k][j], h[k][j], dot);
+                const float hn = hv[j] * rstd;
+                if (live) dw[k][j] = fmaf(gv[j], hn, dw[k][j]);
+                dot = fmaf(gv[j] * wv[j], hn, dot);
             }
         }
         dot = row_sum<ROWT>(dot, shared) / (float)a.N;
@@ -200,10 +241,13 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_grad_kernel(cons
 #pragma unroll
         for (int k = 0; k < VPT; ++k) {
             const int c = (k * ROWT + t) * 8;
-            float g[8] = {};
-            if (a.gh) row8<DT>(a.gh, rw * a.ldgh, c, a.N, g);
+            float hv[8], gv[8], wv[8], g[8] = {};
+            h[k].put(hv);
+            gy[k].put(gv);
+            w[k].put(wv);
+            if (a.gh) gh[k].put(g);
 #pragma unroll
-            for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, fmaf(-dot, h[k][j], n[k][j]), g[j]);
+            for (int j = 0; j < 8; ++j) g[j] = fmaf(rstd, fmaf(-dot, hv[j] * rstd, gv[j] * wv[j]), g[j]);
             if (live && c < a.N) put8<DT>(a.dx, row * a.lddx, c, a.N, g);
         }
     }
