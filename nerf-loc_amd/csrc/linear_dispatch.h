@@ -37,8 +37,7 @@ int gemm_tiles(GemmArgs& g, hipStream_t s) {
         return launch<DT, ODT, LAY, 64, 64, 2, 2, REGS>(g, s);
     }
     if constexpr (LAY != DW && elem_size(DT) == 2) {
-        const bool narrow = g.Q <= 128 || g.seg[0].red <= 128;
-        if (g.nseg == 1 && !g.partial && g.Q <= 256 && g.seg[0].red <= 256 && g.P >= (narrow ? 65536 : 131072)) return launch_rows<DT, LAY == DX>(g, s);
+        if (rows_ok(g)) return launch_rows<DT, LAY == DX>(g, s);
     }
     const long long red = g.splits > 1 ? g.red_part : g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0);
     const bool deep = red * elem_size(DT) >= 16 * 128;

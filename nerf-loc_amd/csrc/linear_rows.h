@@ -8,12 +8,21 @@
 // one row per fragment; two fragments are turned into 8 consecutive columns per lane (64 bytes of each row per store) by
 // two permlane swaps.
 #pragma once
+#include <utility>
+
 #include "linear.h"
 
 namespace nerf {
 namespace lin {
 
 typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+
+// f(0), f(1), ... f(N - 1) with constant arguments: arrays indexed by them stay in registers, where a loop that the
+// compiler unrolls late can leave them in scratch memory
+template <class F, int... I>
+__device__ __forceinline__ void each_of(F&& f, std::integer_sequence<int, I...>) { (f(std::integral_constant<int, I>{}), ...); }
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) { each_of(f, std::make_integer_sequence<int, N>{}); }
 
 // Two fragments' columns of a row: lane group g holds 4 columns of each, 16 f + 4 g .. + 4.  Afterwards (or before, the
 // exchange undoes itself when run backwards) it holds 8 consecutive ones, 8 g .. + 8.  A swap exchanges a bit of the
@@ -53,28 +62,17 @@ __device__ __forceinline__ void unpack2(unsigned v, float& a, float& b) {
     }
 }
 
-// The packed columns of two fragments (lo: the first two of a lane's four, hi: the others) to or from 8 g .. + 8 of the
-// row's 32 at p; n: columns left from there.
-__device__ __forceinline__ void store_row(unsigned (&lo)[2], unsigned (&hi)[2], unsigned short* p, long long n) {
+// The packed columns of two fragments (lo: the first two of a lane's four, hi: the others) and the 16 bytes 8 g .. + 8 of
+// the row's 32 columns.
+__device__ __forceinline__ u32x4 to_row(unsigned (&lo)[2], unsigned (&hi)[2]) {
     swap32(lo[0], lo[1]);
     swap32(hi[0], hi[1]);
     swap16(lo[0], lo[1]);
     swap16(hi[0], hi[1]);
-    const unsigned w[4] = {lo[0], hi[0], lo[1], hi[1]};
-    if (n >= 8) __builtin_memcpy(p, w, 16);
-    else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) p[j] = (unsigned short)(w[j >> 1] >> (16 * (j & 1)));
-    }
+    return u32x4{lo[0], hi[0], lo[1], hi[1]};
 }
-__device__ __forceinline__ void load_row(unsigned (&lo)[2], unsigned (&hi)[2], const unsigned short* p, long long n) {
-    unsigned w[4] = {0, 0, 0, 0};
-    if (n >= 8) __builtin_memcpy(w, p, 16);
-    else {
-#pragma unroll
-        for (int j = 0; j < 8; ++j) if (j < n) w[j >> 1] |= (unsigned)p[j] << (16 * (j & 1));
-    }
-    lo[0] = w[0]; hi[0] = w[1]; lo[1] = w[2]; hi[1] = w[3];
+__device__ __forceinline__ void from_row(const u32x4& v, unsigned (&lo)[2], unsigned (&hi)[2]) {
+    lo[0] = v[0]; hi[0] = v[1]; lo[1] = v[2]; hi[1] = v[3];
     swap16(lo[0], lo[1]);
     swap16(hi[0], hi[1]);
     swap32(lo[0], lo[1]);
@@ -83,8 +81,13 @@ __device__ __forceinline__ void load_row(unsigned (&lo)[2], unsigned (&hi)[2], c
 
 // H x NF 16-column fragments of C, KS 32-element steps of the reduction; TB: B lies reduction-major.  With H = 2 two waves
 // share the rows and halve the columns: 32 rows x 256 columns of sums, 256 inputs of 32 rows and the weights' fragments
-// do not fit one wave's 256 registers (measured with spills: 310 us for 786432 x 256 x 256).
-template <int DT, int NF, int KS, int RF, int H, bool TB>
+// do not fit one wave's 256 registers (measured with spills: 310 us for 786432 x 256 x 256).  Z, RES: the epilogue stores
+// its argument, adds a residual.
+//
+// From a block's first load to its last store there is no branch: loads and stores retire in order, and behind a branch
+// that may or may not have issued some the compiler waits as if it had issued none, that is, for the stores of the block
+// before.  What lies outside the matrices is masked by offsets outside the buffers instead.
+template <int DT, int NF, int KS, int RF, int H, bool TB, bool Z, bool RES>
 __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
     static_assert(NF % 2 == 0 && KS >= 2 && elem_size(DT) == 2, "whole pairs of fragments, whole swizzled rows");
     constexpr int ROWB = KS * 64, ROWS = RF * 16;
@@ -103,26 +106,29 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
     const void* at = nullptr;
     unsigned off[RF];
     auto aim = [&](long long blk) {
+        // behind the last block nothing is inside: no branch may stand between the loads, it would make the compiler wait
+        // for all of them
         const long long p0 = blk * ROWS, left = g.P - p0;
-        at = static_cast<const char*>(g.seg[0].a) + p0 * lda * 2;
+        at = left > 0 ? static_cast<const char*>(g.seg[0].a) + p0 * lda * 2 : static_cast<const char*>(g.seg[0].a);
 #pragma unroll
         for (int r = 0; r < RF; ++r) off[r] = r * 16 + i < left ? row_off[r] : OUTSIDE;
     };
-    auto fetch = [&](int s) {
+    const int kleft = K - gr * 8;
+    // eight columns of a row of y, z or the residual: its offset from the block's first row
+    auto spot = [&](long long p0, long long ld, int r, int J) {
+        const int q = half + J * 16 + gr * 8;
+        return p0 + r * 16 + i < g.P && q < Q ? (unsigned)((r * 16 + i) * (int)ld + q) * 2 : OUTSIDE;
+    };
+    auto rows_of = [&](const void* p, long long p0, long long ld) {
+        return __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(const_cast<void*>(p)) + p0 * ld * 2, 0, 0x7fffffff, 0x00020000);
+    };
+    auto fetch = [&](int r, int s) {
         const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(at), 0, 0x7fffffff, 0x00020000);
-#pragma unroll
-        for (int r = 0; r < RF; ++r) {
-            unsigned o = off[r];
-            if (s * 32 + 32 > K && s * 32 + gr * 8 >= K) o = OUTSIDE;
-            x[r][s] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o, s * 64, 0));
-        }
+        return __builtin_amdgcn_raw_buffer_load_b128(rs, s * 32 < kleft ? off[r] : OUTSIDE, s * 64, 0);
     };
     long long blk = (long long)blockIdx.x * (8 / H) + wave / H;
-    if (blk < blocks) {
-        aim(blk);
-#pragma unroll
-        for (int s = 0; s < KS; ++s) fetch(s);
-    }
+    aim(blk);
+    each<KS>([&](auto s) { each<RF>([&](auto r) { x[r][s] = fetch(r, s); }); });
 
     // weights: row q of LDS holds B(q, 0 .. 32 KS), chunk c of each eight at c ^ (q & 7); zeros outside the matrix
     if constexpr (!TB) {
@@ -158,84 +164,94 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
     __syncthreads();
 
     const unsigned char* wl = wlds + (half + i) * ROWB;
-    // a step's weight fragments are read while the step before it is worked on; the first step's are those of every block
-    i32x4 w[2][NF];
+    // a step's weight fragments are read while the step before it is worked on, the first step's at the last one; with a
+    // residual, whose rows take the registers, right before their use
+    constexpr int WB = RES ? 1 : 2;
+    i32x4 w[WB][NF];
     auto weights = [&](int s) {
         const int place = ((4 * s & ~7) | (((4 * s + gr) & 7) ^ (i & 7))) * 16;
 #pragma unroll
-        for (int j = 0; j < NF; ++j) w[s & 1][j] = *reinterpret_cast<const i32x4*>(wl + j * 16 * ROWB + place);
+        for (int j = 0; j < NF; ++j) w[s % WB][j] = *reinterpret_cast<const i32x4*>(wl + j * 16 * ROWB + place);
     };
     static_assert(KS % 2 == 0, "the first step's fragments follow the last one's");
-    weights(0);
+    if constexpr (!RES) weights(0);
     for (; blk < blocks; blk += stride) {
-        const bool more = blk + stride < blocks;
-        if (more) aim(blk + stride);
+        const long long p0 = blk * ROWS;
+        aim(blk + stride);
+        u32x4 res[RES ? RF : 1][RES ? NF / 2 : 1];
+        if constexpr (RES) {
+            const auto rs = rows_of(g.res, p0, g.ldr);
+#pragma unroll
+            for (int r = 0; r < RF; ++r)
+#pragma unroll
+                for (int J = 0; J < NF; J += 2)
+                    res[r][J / 2] = __builtin_bit_cast(u32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, spot(p0, g.ldr, r, J), 0, 0));
+        }
         f32x4 acc[RF][NF];
-#pragma unroll
-        for (int j = 0; j < NF; ++j) {
+        each<NF>([&](auto j) {
             const f32x4 b = *reinterpret_cast<const f32x4*>(blds + half + j * 16 + gr * 4);
-#pragma unroll
-            for (int r = 0; r < RF; ++r) acc[r][j] = b;
-        }
-#pragma unroll
-        for (int s = 0; s < KS; ++s) {
-            weights((s + 1) % KS);
+            each<RF>([&](auto r) { acc[r][j] = b; });
+        });
+        each<KS>([&](auto s) {
+            weights(RES ? int(s) : (s + 1) % KS);
             __builtin_amdgcn_sched_barrier(0);
-#pragma unroll
-            for (int j = 0; j < NF; ++j)
-#pragma unroll
-                for (int r = 0; r < RF; ++r) mma<DT>(acc[r][j], w[s & 1][j], __builtin_bit_cast(i32x4, x[r][s]));
-            if (more) fetch(s);
+            each<NF>([&](auto j) { each<RF>([&](auto r) { mma<DT>(acc[r][j], w[s % WB][j], __builtin_bit_cast(i32x4, x[r][s])); }); });
+            each<RF>([&](auto r) { x[r][s] = fetch(r, s); });
             __builtin_amdgcn_sched_barrier(0);
+        });
+        auto pack = [](const f32x4& a, const f32x4& b, unsigned (&lo)[2], unsigned (&hi)[2]) {
+            lo[0] = pack2<DT>(a[0], a[1]);
+            hi[0] = pack2<DT>(a[2], a[3]);
+            lo[1] = pack2<DT>(b[0], b[1]);
+            hi[1] = pack2<DT>(b[2], b[3]);
+        };
+        if constexpr (Z) {
+            const auto rs = rows_of(g.z, p0, g.ldz);
+            each<RF>([&](auto r) {
+                each<NF / 2>([&](auto J) {
+                    unsigned lo[2], hi[2];
+                    pack(acc[r][2 * J], acc[r][2 * J + 1], lo, hi);
+                    __builtin_amdgcn_raw_buffer_store_b128(to_row(lo, hi), rs, spot(p0, g.ldz, r, 2 * J), 0, 0);
+                });
+            });
         }
-#pragma unroll
-        for (int r = 0; r < RF; ++r) {
-            const long long p = blk * ROWS + r * 16 + i;
-            const bool live = p < g.P;
-#pragma unroll
-            for (int J = 0; J < NF; J += 2) {
-                const long long q = half + J * 16 + gr * 8, n = live ? g.Q - q : 0;
+        const auto rs = rows_of(g.y, p0, g.ldy);
+        each<RF>([&](auto r) {
+            each<NF / 2>([&](auto J) {
+                f32x4 v[2] = {acc[r][2 * J], acc[r][2 * J + 1]};
                 unsigned lo[2], hi[2];
-                f32x4 v[2] = {acc[r][J], acc[r][J + 1]};
-                auto pack = [&] {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) { lo[j] = pack2<DT>(v[j][0], v[j][1]); hi[j] = pack2<DT>(v[j][2], v[j][3]); }
-                };
-                auto apply = [&](int act) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j)
-#pragma unroll
-                        for (int k = 0; k < 4; ++k) v[j][k] = act_fn(v[j][k], act);
-                };
-                if (g.z) {
-                    pack();
-                    store_row(lo, hi, static_cast<unsigned short*>(g.z) + p * g.ldz + q, n);
-                }
-                if (g.act == NERF_ACT_RELU) apply(NERF_ACT_RELU);
-                else if (g.act == NERF_ACT_GELU) apply(NERF_ACT_GELU);
-                else if (g.act == NERF_ACT_SILU) apply(NERF_ACT_SILU);
-                if (g.res) {
-                    load_row(lo, hi, static_cast<const unsigned short*>(g.res) + p * g.ldr + q, n);
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        float a, b;
+                each<2>([&](auto j) {
+                    f32x4 t = v[j];
+                    if (g.act == NERF_ACT_RELU) t = f32x4{act_fn(t[0], NERF_ACT_RELU), act_fn(t[1], NERF_ACT_RELU), act_fn(t[2], NERF_ACT_RELU), act_fn(t[3], NERF_ACT_RELU)};
+                    else if (g.act == NERF_ACT_GELU) t = f32x4{act_fn(t[0], NERF_ACT_GELU), act_fn(t[1], NERF_ACT_GELU), act_fn(t[2], NERF_ACT_GELU), act_fn(t[3], NERF_ACT_GELU)};
+                    else if (g.act == NERF_ACT_SILU) t = f32x4{act_fn(t[0], NERF_ACT_SILU), act_fn(t[1], NERF_ACT_SILU), act_fn(t[2], NERF_ACT_SILU), act_fn(t[3], NERF_ACT_SILU)};
+                    v[j] = t;
+                });
+                if constexpr (RES) {
+                    from_row(res[r][J], lo, hi);
+                    each<2>([&](auto j) {
+                        float a, b, c, d;
                         unpack2<DT>(lo[j], a, b);
-                        v[j][0] += a; v[j][1] += b;
-                        unpack2<DT>(hi[j], a, b);
-                        v[j][2] += a; v[j][3] += b;
-                    }
+                        unpack2<DT>(hi[j], c, d);
+                        v[j] += f32x4{a, b, c, d};
+                    });
                 }
-                pack();
-                store_row(lo, hi, static_cast<unsigned short*>(g.y) + p * g.ldy + q, n);
-            }
-        }
+                pack(v[0], v[1], lo, hi);
+                __builtin_amdgcn_raw_buffer_store_b128(to_row(lo, hi), rs, spot(p0, g.ldy, r, 2 * J), 0, 0);
+            });
+        });
     }
 }
 
 template <int DT, bool TB, int NF, int H, int KS>
 int launch_rows2(GemmArgs& g, hipStream_t s) {
     const long long rows = 8 / H * 32, groups = (g.P + rows - 1) / rows;
-    hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB>), dim3((unsigned)(groups < 256 ? groups : 256)), dim3(512), 0, s, g);
+    const dim3 grid((unsigned)(groups < 256 ? groups : 256));
+    if constexpr (TB) hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB, false, false>), grid, dim3(512), 0, s, g);
+    else if (g.z && g.res) hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB, true, true>), grid, dim3(512), 0, s, g);
+    else if (g.z) hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB, true, false>), grid, dim3(512), 0, s, g);
+    else if (g.res) hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB, false, true>), grid, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((rows_kernel<DT, NF, KS, 2, H, TB, false, false>), grid, dim3(512), 0, s, g);
     NERF_LAUNCH_CHECK();
     return NERF_OK;
 }
@@ -245,6 +261,14 @@ int launch_rows1(GemmArgs& g, hipStream_t s) {
     if (k <= 64) return launch_rows2<DT, TB, NF, H, 2>(g, s);
     if (k <= 128) return launch_rows2<DT, TB, NF, H, 4>(g, s);
     return launch_rows2<DT, TB, NF, H, 8>(g, s);
+}
+// Whether the streaming kernel takes a product: enough rows to keep every wave going, both sides within its registers and
+// LDS, outputs in whole 16-byte groups.
+inline bool rows_ok(const GemmArgs& g) {
+    const long long k = g.seg[0].red;
+    if (g.nseg != 1 || g.partial || g.Q > 256 || k > 256 || g.Q % 8 || g.P < (g.Q <= 128 || k <= 128 ? 65536 : 131072)) return false;
+    auto rows = [](const void* p, long long ld) { return !p || (((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld < (1ll << 24)); };
+    return rows(g.y, g.ldy) && rows(g.z, g.ldz) && rows(g.res, g.ldr);
 }
 template <int DT, bool TB>
 int launch_rows(GemmArgs& g, hipStream_t s) {
