@@ -243,6 +243,160 @@ __global__ void __launch_bounds__(512) rows_kernel(const GemmArgs g) {
     }
 }
 
+// ---------------------------------------------------------------------------------------------- 129 to 256 outputs
+// The same with the sides exchanged: a wave keeps 64 columns of the weights in registers (32 fragments at 256 inputs) and
+// the samples come through LDS, where all four column groups find them, 64 rows a stage and several stages under way:
+// the loads in flight are no longer what the registers hold.  (rows_kernel on 786432 x 256 x 256 bf16: 212 us, of which
+// the products alone take 84, with the loads 141, with the stores 104.)
+//
+// Everything a wave asks of memory inside the loop is counted: D loads to LDS and E stores a stage, issued without a
+// branch, so stage t has landed once all but the E + (S - 2)(D + E) youngest are done.
+template <int DT, int KS, bool TB, bool Z>
+__global__ void __launch_bounds__(512) panel_kernel(const GemmArgs g) {
+    constexpr int ROWC = KS * 4, ROWB = KS * 64, TILE = 64, STAGE = TILE * ROWB;
+    constexpr int S = KS == 8 ? 4 : KS == 4 ? 6 : 8;
+    constexpr int D = TILE * ROWC / 512, E = Z ? 8 : 4, YOUNGER = E + (S - 2) * (D + E);
+    static_assert(D * 512 == TILE * ROWC && YOUNGER < 64 && 256 * ROWB <= S * STAGE && S * STAGE <= 128 * 1024, "stages");
+    __shared__ __align__(1024) unsigned char smem[S * STAGE];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), i = lane & 15, gr = lane >> 4;
+    const int q0 = (wave & 3) * 64, r0 = (wave >> 2) * 32;       // this wave's columns and rows of a tile
+    const int Q = (int)g.Q, K = (int)g.seg[0].red;
+    const long long lda = g.seg[0].lda, tiles = (g.P + TILE - 1) / TILE;
+    const unsigned lds0 = (unsigned)(unsigned long long)(lds_u8*)smem;
+
+    // chunk c of row p of a tile sits at c ^ (p & 7); lane L of the tile's loads fetches what belongs at its place
+    unsigned off[D];
+    int row[D];
+    each<D>([&](auto d) {
+        const int L = d * 512 + tid, slot = L % ROWC;
+        row[d] = L / ROWC;
+        const int c = (slot & ~7) | ((slot ^ row[d]) & 7);
+        off[d] = c * 8 < K ? (unsigned)(row[d] * (int)lda + c * 8) * 2 : OUTSIDE;
+    });
+    auto fetch = [&](long long t, int stage) {
+        const long long p0 = t * TILE, left = g.P - p0;          // behind the last tile: nothing is inside
+        const i32x4 rsrc = buffer_of(static_cast<const char*>(g.seg[0].a) + (left > 0 ? p0 * lda * 2 : 0));
+        const unsigned at = lds0 + stage * STAGE + wave * 1024;
+        each<D>([&](auto d) { dma16(at + d * 8192, row[d] < left ? off[d] : OUTSIDE, rsrc); });
+    };
+
+    i32x4 w[KS][4];
+    f32x4 bias[4];
+    long long t = blockIdx.x;
+    if constexpr (!TB) {
+        each<S - 1>([&](auto k) { fetch(t + k * (long long)gridDim.x, k); });
+        const auto rs = __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(g.seg[0].b), 0, 0x7fffffff, 0x00020000);
+        each<KS>([&](auto s) {
+            each<4>([&](auto j) {
+                const int q = q0 + j * 16 + i, r = s * 32 + gr * 8;
+                const unsigned o = q < Q && r < K ? (unsigned)(q * (int)g.seg[0].ldb + r) * 2 : OUTSIDE;
+                w[s][j] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(rs, o, 0, 0));
+            });
+        });
+    } else {
+        // through LDS, turned in registers 8 x 8 at a time
+        for (int k = tid; k < 32 * ROWC; k += 512) {
+            const int c = k / 32, q = k % 32 * 8;
+            unsigned in[8][4];
+#pragma unroll
+            for (int r = 0; r < 8; ++r) {
+                uint4 v = make_uint4(0, 0, 0, 0);
+                if (c * 8 + r < K && q < Q) v = *reinterpret_cast<const uint4*>(static_cast<const char*>(g.seg[0].b) + ((long long)(c * 8 + r) * g.seg[0].ldb + q) * 2);
+                in[r][0] = v.x; in[r][1] = v.y; in[r][2] = v.z; in[r][3] = v.w;
+            }
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                unsigned out[4];
+#pragma unroll
+                for (int m = 0; m < 4; ++m)
+                    out[m] = __builtin_amdgcn_perm(in[2 * m + 1][j >> 1], in[2 * m][j >> 1], j & 1 ? 0x07060302 : 0x05040100);
+                *reinterpret_cast<uint4*>(smem + (q + j) * ROWB + ((c & ~7) | ((c ^ (q + j)) & 7)) * 16) = make_uint4(out[0], out[1], out[2], out[3]);
+            }
+        }
+        __syncthreads();
+        each<KS>([&](auto s) {
+            each<4>([&](auto j) {
+                const int c = 4 * s + gr, q = q0 + j * 16 + i;
+                w[s][j] = *reinterpret_cast<const i32x4*>(smem + q * ROWB + ((c & ~7) | ((c ^ q) & 7)) * 16);
+            });
+        });
+        __syncthreads();
+        each<S - 1>([&](auto k) { fetch(t + k * (long long)gridDim.x, k); });
+    }
+    each<4>([&](auto j) {
+        const int q = q0 + j * 16 + gr * 4;
+        auto b = [&](int k) { return g.bias && q + k < Q ? ld_elem(g.bias, q + k, DT) : 0.f; };
+        bias[j] = f32x4{b(0), b(1), b(2), b(3)};
+    });
+    // the weights and the bias have arrived (and with them, once, the first stages): from here on the count is the loop's
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+
+    const unsigned char* frag = smem + (r0 + i) * ROWB;
+    int stage = 0;
+    for (; t < tiles; t += gridDim.x) {
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(YOUNGER) : "memory");
+        __builtin_amdgcn_fence(__ATOMIC_RELEASE, "workgroup", "local");
+        __builtin_amdgcn_s_barrier();
+        __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "workgroup", "local");
+        // every wave has read the stage before this one: it takes the tile S - 1 ahead
+        fetch(t + (S - 1) * (long long)gridDim.x, stage == 0 ? S - 1 : stage - 1);
+        f32x4 acc[2][4];
+        each<4>([&](auto j) { each<2>([&](auto r) { acc[r][j] = bias[j]; }); });
+        const unsigned char* x = frag + stage * STAGE;
+        each<KS>([&](auto s) {
+            const int place = ((4 * s & ~7) | (((4 * s + gr) & 7) ^ (i & 7))) * 16;
+            i32x4 a[2];
+            each<2>([&](auto r) { a[r] = *reinterpret_cast<const i32x4*>(x + r * 16 * ROWB + place); });
+            each<4>([&](auto j) { each<2>([&](auto r) { mma<DT>(acc[r][j], w[s][j], a[r]); }); });
+        });
+        const long long p0 = t * TILE + r0;
+        auto out = [&](void* base, long long ld) {
+            const auto rs = __builtin_amdgcn_make_buffer_rsrc(static_cast<char*>(base) + p0 * ld * 2, 0, 0x7fffffff, 0x00020000);
+            each<2>([&](auto r) {
+                each<2>([&](auto J) {
+                    const f32x4 &u = acc[r][2 * J], &v = acc[r][2 * J + 1];
+                    unsigned lo[2] = {pack2<DT>(u[0], u[1]), pack2<DT>(v[0], v[1])}, hi[2] = {pack2<DT>(u[2], u[3]), pack2<DT>(v[2], v[3])};
+                    const int q = q0 + J * 32 + gr * 8;
+                    const unsigned o = p0 + r * 16 + i < g.P && q < Q ? (unsigned)((r * 16 + i) * (int)ld + q) * 2 : OUTSIDE;
+                    __builtin_amdgcn_raw_buffer_store_b128(to_row(lo, hi), rs, o, 0, 0);
+                });
+            });
+        };
+        if constexpr (Z) out(g.z, g.ldz);
+        each<2>([&](auto r) {
+            each<4>([&](auto j) {
+                f32x4 v = acc[r][j];
+                if (g.act == NERF_ACT_RELU) v = f32x4{act_fn(v[0], NERF_ACT_RELU), act_fn(v[1], NERF_ACT_RELU), act_fn(v[2], NERF_ACT_RELU), act_fn(v[3], NERF_ACT_RELU)};
+                else if (g.act == NERF_ACT_GELU) v = f32x4{act_fn(v[0], NERF_ACT_GELU), act_fn(v[1], NERF_ACT_GELU), act_fn(v[2], NERF_ACT_GELU), act_fn(v[3], NERF_ACT_GELU)};
+                else if (g.act == NERF_ACT_SILU) v = f32x4{act_fn(v[0], NERF_ACT_SILU), act_fn(v[1], NERF_ACT_SILU), act_fn(v[2], NERF_ACT_SILU), act_fn(v[3], NERF_ACT_SILU)};
+                acc[r][j] = v;
+            });
+        });
+        out(g.y, g.ldy);
+        stage = stage + 1 == S ? 0 : stage + 1;
+    }
+    // the loads behind the last tile write (zeros) to this workgroup's LDS: they end before it does
+    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+}
+
+template <int DT, bool TB, int KS>
+int launch_panel1(GemmArgs& g, hipStream_t s) {
+    const long long tiles = (g.P + 63) / 64;
+    const dim3 grid((unsigned)(tiles < 256 ? tiles : 256));
+    if constexpr (TB) hipLaunchKernelGGL((panel_kernel<DT, KS, TB, false>), grid, dim3(512), 0, s, g);
+    else if (g.z) hipLaunchKernelGGL((panel_kernel<DT, KS, TB, true>), grid, dim3(512), 0, s, g);
+    else hipLaunchKernelGGL((panel_kernel<DT, KS, TB, false>), grid, dim3(512), 0, s, g);
+    NERF_LAUNCH_CHECK();
+    return NERF_OK;
+}
+template <int DT, bool TB>
+int launch_panel(GemmArgs& g, hipStream_t s) {
+    const long long k = g.seg[0].red;
+    if (k <= 64) return launch_panel1<DT, TB, 2>(g, s);
+    if (k <= 128) return launch_panel1<DT, TB, 4>(g, s);
+    return launch_panel1<DT, TB, 8>(g, s);
+}
+
 template <int DT, bool TB, int NF, int H, int KS>
 int launch_rows2(GemmArgs& g, hipStream_t s) {
     const long long rows = 8 / H * 32, groups = (g.P + rows - 1) / rows;
@@ -274,6 +428,7 @@ template <int DT, bool TB>
 int launch_rows(GemmArgs& g, hipStream_t s) {
     if (g.Q <= 64) return launch_rows1<DT, TB, 4, 1>(g, s);
     if (g.Q <= 128) return launch_rows1<DT, TB, 8, 1>(g, s);
+    if (!g.res) return launch_panel<DT, TB>(g, s);
     return launch_rows1<DT, TB, 8, 2>(g, s);
 }
 
