@@ -140,17 +140,30 @@ __global__ void __launch_bounds__(256) finish_kernel(const GemmArgs g, int parts
     epilogue8<DT, SCALED>(g, p, q, v);
 }
 
-// Rows copied to places on 16 bytes, zeros behind their ends to a whole chunk.  One chunk a thread.
+// Rows copied to places on 16 bytes, zeros behind their ends to a whole chunk: all the operands of a product that need it
+// in one launch, one chunk a thread.
+struct PackArgs {
+    struct Job {
+        const char* src;
+        uint4* dst;
+        long long ld, rows, cols, chunks;        // chunks: of a row
+        unsigned first;                          // workgroup
+    } job[4];
+    int jobs;
+};
 template <int E>
-__global__ void __launch_bounds__(256) pack_kernel(const char* src, long long ld, long long rows, long long cols, uint4* dst, long long chunks) {
+__global__ void __launch_bounds__(256) pack_kernel(const PackArgs a) {
     constexpr int CE = 16 / E;
-    const long long t = (long long)blockIdx.x * 256 + threadIdx.x, row = t / chunks, c = t % chunks * CE;
-    if (row >= rows) return;
+    int n = 0;
+    while (n + 1 < a.jobs && blockIdx.x >= a.job[n + 1].first) ++n;
+    const PackArgs::Job& j = a.job[n];
+    const long long t = (long long)(blockIdx.x - j.first) * 256 + threadIdx.x, row = t / j.chunks, c = t % j.chunks * CE;
+    if (row >= j.rows) return;
     uint4 v;
-    const char* p = src + (row * ld + c) * E;
-    if (c + CE <= cols) __builtin_memcpy(&v, p, 16);
-    else v = part_chunk<E>(p, (int)(cols - c));
-    dst[t] = v;
+    const char* p = j.src + (row * j.ld + c) * E;
+    if (c + CE <= j.cols) __builtin_memcpy(&v, p, 16);
+    else v = part_chunk<E>(p, (int)(j.cols - c));
+    j.dst[t] = v;
 }
 
 static int dispatch_gemm(int dtype, int layout, GemmArgs& g, hipStream_t s) {
@@ -175,20 +188,7 @@ struct Mat {
 static bool dma_rows(const Mat& m, int e) { return ((uintptr_t)m.p & 15) == 0 && (m.ld * e) % 16 == 0 && (m.padded || (m.cols * e) % 16 == 0); }
 static long long packed_ld(long long cols, int e) { return (cols * e + 15) / 16 * 16 / e; }
 static size_t packed_bytes(const Mat& m, int e) { return align256((size_t)m.rows * packed_ld(m.cols, e) * e); }
-static int pack(Mat& m, int e, char* to, hipStream_t s) {
-    const long long ldd = packed_ld(m.cols, e), chunks = ldd * e / 16;
-    const dim3 grid((unsigned)((m.rows * chunks + 255) / 256));
-    const char* src = static_cast<const char*>(m.p);
-    uint4* dst = reinterpret_cast<uint4*>(to);
-    if (e == 4) hipLaunchKernelGGL(pack_kernel<4>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
-    else if (e == 2) hipLaunchKernelGGL(pack_kernel<2>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
-    else hipLaunchKernelGGL(pack_kernel<1>, grid, dim3(256), 0, s, src, m.ld, m.rows, m.cols, dst, chunks);
-    NERF_LAUNCH_CHECK();
-    m.p = to;
-    m.ld = ldd;
-    m.padded = true;
-    return NERF_OK;
-}
+static long long packed_groups(const Mat& m, int e) { return (m.rows * (packed_ld(m.cols, e) * e / 16) + 255) / 256; }
 
 // One product with its copies and its split: what it takes of the workspace, and the launches.
 struct Product {
@@ -206,14 +206,19 @@ struct Product {
     bool packs() const {
         const int e = elem_size(dtype);
         double copy_us = 0, products = 0;
+        long long groups = 0;
         for (int s = 0; s < nseg; ++s) {
             products += (double)P * Q * red[s];
             for (const Mat& m : {a[s], b[s]}) {
                 if (m.rows >= (1ll << 31) || m.cols * e >= (1ll << 22)) return false;
-                if (!dma_rows(m, e)) copy_us += 4 + (double)m.rows * m.cols * e * 2 / 5e6;
+                if (!dma_rows(m, e)) {
+                    copy_us += (double)m.rows * m.cols * e * 2 / 5e6;
+                    groups += packed_groups(m, e);
+                }
             }
         }
-        if (copy_us == 0 || (layout == FWD && P <= FEW_ROWS)) return false;
+        if (groups == 0 || groups >= (1ll << 31) || (layout == FWD && P <= FEW_ROWS)) return false;
+        copy_us += 5;
         const double aligned_us = products * 2 / (dtype == F32 ? 130e6 : 700e6);
         return copy_us < aligned_us * (dtype == F32 ? 0.4 : layout == FWD ? 1 : 4);
     }
@@ -233,15 +238,26 @@ struct Product {
     // given: parts that the caller has set up and will add up itself (g.partial, g.red_part)
     int run(GemmArgs& g, char* ws, hipStream_t st, int given = 1) {
         const int e = elem_size(dtype), sp = splits();
-        if (packs())
+        if (packs()) {
+            PackArgs pa = {};
+            long long groups = 0;
             for (int s = 0; s < nseg; ++s)
                 for (Mat* m : {&a[s], &b[s]})
                     if (!dma_rows(*m, e)) {
-                        const size_t n = packed_bytes(*m, e);
-                        const int rc = pack(*m, e, ws, st);
-                        if (rc != NERF_OK) return rc;
-                        ws += n;
+                        const long long ldd = packed_ld(m->cols, e);
+                        pa.job[pa.jobs++] = {static_cast<const char*>(m->p), reinterpret_cast<uint4*>(ws), m->ld, m->rows, m->cols, ldd * e / 16, (unsigned)groups};
+                        groups += packed_groups(*m, e);
+                        m->p = ws;
+                        ws += packed_bytes(*m, e);
+                        m->ld = ldd;
+                        m->padded = true;
                     }
+            const dim3 grid((unsigned)groups);
+            if (e == 4) hipLaunchKernelGGL(pack_kernel<4>, grid, dim3(256), 0, st, pa);
+            else if (e == 2) hipLaunchKernelGGL(pack_kernel<2>, grid, dim3(256), 0, st, pa);
+            else hipLaunchKernelGGL(pack_kernel<1>, grid, dim3(256), 0, st, pa);
+            NERF_LAUNCH_CHECK();
+        }
         for (int s = 0; s < nseg; ++s) g.seg[s] = {a[s].p, b[s].p, a[s].ld, b[s].ld, red[s], a[s].padded, b[s].padded};
         g.nseg = nseg;
         g.P = P;

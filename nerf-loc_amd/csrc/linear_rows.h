@@ -363,15 +363,17 @@ __global__ void __launch_bounds__(512) panel_kernel(const GemmArgs g) {
             });
         };
         if constexpr (Z) out(g.z, g.ldz);
-        each<2>([&](auto r) {
-            each<4>([&](auto j) {
-                f32x4 v = acc[r][j];
-                if (g.act == NERF_ACT_RELU) v = f32x4{act_fn(v[0], NERF_ACT_RELU), act_fn(v[1], NERF_ACT_RELU), act_fn(v[2], NERF_ACT_RELU), act_fn(v[3], NERF_ACT_RELU)};
-                else if (g.act == NERF_ACT_GELU) v = f32x4{act_fn(v[0], NERF_ACT_GELU), act_fn(v[1], NERF_ACT_GELU), act_fn(v[2], NERF_ACT_GELU), act_fn(v[3], NERF_ACT_GELU)};
-                else if (g.act == NERF_ACT_SILU) v = f32x4{act_fn(v[0], NERF_ACT_SILU), act_fn(v[1], NERF_ACT_SILU), act_fn(v[2], NERF_ACT_SILU), act_fn(v[3], NERF_ACT_SILU)};
-                acc[r][j] = v;
+        auto apply = [&](auto act) {
+            each<2>([&](auto r) {
+                each<4>([&](auto j) {
+                    const f32x4 v = acc[r][j];
+                    acc[r][j] = f32x4{act_fn(v[0], act), act_fn(v[1], act), act_fn(v[2], act), act_fn(v[3], act)};
+                });
             });
-        });
+        };
+        if (g.act == NERF_ACT_RELU) apply(std::integral_constant<int, NERF_ACT_RELU>{});
+        else if (g.act == NERF_ACT_GELU) apply(std::integral_constant<int, NERF_ACT_GELU>{});
+        else if (g.act == NERF_ACT_SILU) apply(std::integral_constant<int, NERF_ACT_SILU>{});
         out(g.y, g.ldy);
         stage = stage + 1 == S ? 0 : stage + 1;
     }

@@ -686,6 +686,11 @@ FEW_ROWS = 64            # up to here the forward products take no workspace
 
 
 _CALLS = {}
+_RAW_STREAM = getattr(torch._C, "_cuda_getCurrentRawStream", None)      # the handle without a Stream object around it
+
+
+def _stream_of(dev):
+    return _RAW_STREAM(dev.index) if _RAW_STREAM is not None else torch.cuda.current_stream(dev).cuda_stream
 
 
 def _call(name, dev, *args):
@@ -695,10 +700,10 @@ def _call(name, dev, *args):
     if fn is None:
         fn = _CALLS[name] = getattr(lib(), name)
     if torch.cuda.current_device() == dev.index:
-        code = fn(*args, torch.cuda.current_stream().cuda_stream)
+        code = fn(*args, _stream_of(dev))
     else:
         with torch.cuda.device(dev):
-            code = fn(*args, torch.cuda.current_stream().cuda_stream)
+            code = fn(*args, _stream_of(dev))
     if code != 0:
         _check(code, name)
 
@@ -784,8 +789,8 @@ def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_
     x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = _layer_input(x0, x1, weight)
     b = None if bias is None else _vector(bias, "bias", N, dt, dev)
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)[:2]
-    y = torch.empty((M, N), dtype=dt, device=dev)
-    z = torch.empty((M, N), dtype=dt, device=dev) if want_z else None
+    y = x0.new_empty((M, N))
+    z = x0.new_empty((M, N)) if want_z else None
     px, p1, pw = x0.data_ptr(), _at(x1), w.data_ptr()
     nbytes = 0 if M <= FEW_ROWS else lib().nerf_linear_workspace_bytes(DTYPES[dt], px, ld0, k0, p1, ld1, k1, pw, ldw, M, N)
     ws = _scratch(nbytes, dev)
@@ -802,7 +807,7 @@ def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=Tru
     g, ldg, _, _ = _matrix(g, "the gradient of y", M, N, dt, dev)
     _need(act == 0 or z is not None, "linear_backward: the gradient through %s needs z", activation)
     zz, ldz = (None, 0) if act == 0 else _matrix(z, "z", M, N, dt, dev)[:2]
-    new = lambda *shape: torch.empty(shape, dtype=dt, device=dev)
+    new = lambda *shape: x0.new_empty(shape)
     dx0 = new(M, k0) if want_x0 else None
     dx1 = new(M, k1) if want_x1 and x1 is not None else None
     dw = new(N, k0 + k1) if want_w else None
@@ -859,8 +864,8 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6, want_h=True, want_rstd=Fals
     x, ldx, M, N, w, r, ldr = _norm_input(x, weight, residual)
     dt, dev = x.dtype, x.device
     _need(float(eps) >= 0.0, "add_rms_norm: eps must not be negative, got %s", eps)
-    h = torch.empty((M, N), dtype=dt, device=dev) if want_h else None
-    y = None if q8 else torch.empty((M, N), dtype=dt, device=dev)
+    h = x.new_empty((M, N)) if want_h else None
+    y = None if q8 else x.new_empty((M, N))
     q = torch.empty((M, N), dtype=torch.float8_e4m3fn, device=dev) if q8 else None
     scale = torch.empty((M,), dtype=torch.float32, device=dev) if q8 else None
     rstd = torch.empty((M,), dtype=torch.float32, device=dev) if want_rstd else None
