@@ -785,16 +785,20 @@ def _layer_input(x0, x1, weight):
 def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_z=False):
     """act([x0 | x1] weight^T + bias) + residual on matrices [M, k0], [M, k1], [N, k0 + k1], [N], [M, N] of one type.
     Returns (y, z): z is the argument of act with want_z, else None."""
-    act = activation_code(activation)
-    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = _layer_input(x0, x1, weight)
+    return _linear(_layer_input(x0, x1, weight), activation_code(activation), bias, residual, want_z)
+
+
+def _linear(operands, act, bias, residual, want_z):
+    """linear on the operands as _layer_input gave them."""
+    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = operands
     b = None if bias is None else _vector(bias, "bias", N, dt, dev)
     r, ldr = (None, 0) if residual is None else _matrix(residual, "residual", M, N, dt, dev)[:2]
     y = x0.new_empty((M, N))
     z = x0.new_empty((M, N)) if want_z else None
-    px, p1, pw = x0.data_ptr(), _at(x1), w.data_ptr()
-    nbytes = 0 if M <= FEW_ROWS else lib().nerf_linear_workspace_bytes(DTYPES[dt], px, ld0, k0, p1, ld1, k1, pw, ldw, M, N)
+    px, p1, pw, code = x0.data_ptr(), _at(x1), w.data_ptr(), DTYPES[dt]
+    nbytes = 0 if M <= FEW_ROWS else lib().nerf_linear_workspace_bytes(code, px, ld0, k0, p1, ld1, k1, pw, ldw, M, N)
     ws = _scratch(nbytes, dev)
-    _call("nerf_linear", dev, DTYPES[dt], px, ld0, k0, p1, ld1, k1, pw, ldw, _at(b), act, _at(r), ldr,
+    _call("nerf_linear", dev, code, px, ld0, k0, p1, ld1, k1, pw, ldw, _at(b), act, _at(r), ldr,
           y.data_ptr(), N, _at(z), N, M, N, _at(ws), nbytes)
     return y, z
 
@@ -802,21 +806,26 @@ def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_
 def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=True, want_x1=True, want_w=True, want_b=True):
     """Gradients of linear for g = dL/dy: (dx0, dx1, dweight, dbias), None where not wanted.  z: the argument of act that
     the forward gave (for relu without a residual, y)."""
-    act = activation_code(activation)
-    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = _layer_input(x0, x1, weight)
+    return _linear_backward(_layer_input(x0, x1, weight), activation_code(activation), g, z, want_x0, want_x1, want_w, want_b)
+
+
+def _linear_backward(operands, act, g, z, want_x0, want_x1, want_w, want_b):
+    x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = operands
     g, ldg, _, _ = _matrix(g, "the gradient of y", M, N, dt, dev)
-    _need(act == 0 or z is not None, "linear_backward: the gradient through %s needs z", activation)
-    zz, ldz = (None, 0) if act == 0 else _matrix(z, "z", M, N, dt, dev)[:2]
-    new = lambda *shape: x0.new_empty(shape)
-    dx0 = new(M, k0) if want_x0 else None
-    dx1 = new(M, k1) if want_x1 and x1 is not None else None
-    dw = new(N, k0 + k1) if want_w else None
-    db = new(N) if want_b else None
-    pg, px, p1, pw = g.data_ptr(), x0.data_ptr(), _at(x1), w.data_ptr()
-    nbytes = lib().nerf_linear_backward_workspace_bytes(DTYPES[dt], pg, ldg, act, px, ld0, k0, p1, ld1, k1, pw, ldw,
+    pz, ldz = None, 0
+    if act != 0:
+        _need(z is not None, "linear_backward: the gradient through the activation needs z")
+        z, ldz, _, _ = _matrix(z, "z", M, N, dt, dev)
+        pz = z.data_ptr()
+    dx0 = x0.new_empty((M, k0)) if want_x0 else None
+    dx1 = x0.new_empty((M, k1)) if want_x1 and x1 is not None else None
+    dw = x0.new_empty((N, k0 + k1)) if want_w else None
+    db = x0.new_empty((N,)) if want_b else None
+    pg, px, p1, pw, code = g.data_ptr(), x0.data_ptr(), _at(x1), w.data_ptr(), DTYPES[dt]
+    nbytes = lib().nerf_linear_backward_workspace_bytes(code, pg, ldg, act, px, ld0, k0, p1, ld1, k1, pw, ldw,
                                                         dx0 is not None, dx1 is not None, dw is not None, M, N)
     ws = _scratch(nbytes, dev)
-    _call("nerf_linear_backward", dev, DTYPES[dt], pg, ldg, _at(zz), ldz, act, px, ld0, k0, p1, ld1, k1, pw, ldw, _at(dx0), k0,
+    _call("nerf_linear_backward", dev, code, pg, ldg, pz, ldz, act, px, ld0, k0, p1, ld1, k1, pw, ldw, _at(dx0), k0,
           _at(dx1), k1, _at(dw), _at(db), M, N, _at(ws), nbytes)
     return dx0, dx1, dw, db
 

@@ -13,7 +13,6 @@ and scratch through torch, and can be captured in a graph.  Gradients are comput
 torch.autocast does not change the types here.
 """
 import torch
-from torch.autograd.function import once_differentiable
 
 from . import hip
 
@@ -41,29 +40,37 @@ def _flat(t, name):
     return t if t.dim() == 2 else t.reshape(t.shape[:-1].numel(), t.shape[-1])
 
 
+def _once(what):
+    # create_graph=True would take the gradients for constants
+    if torch.is_grad_enabled():
+        raise NotImplementedError("%s: the kernels give first derivatives only (create_graph=True asks for the second)" % what)
+
+
 class _LinearFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x0, x1, weight, bias, residual, activation):
-        needs = ctx.needs_input_grad
-        inner = any(needs[:4])
+        operands = hip._layer_input(x0, x1, weight)
+        act = hip.activation_code(activation)
+        n0, n1, nw, nb, _, _ = ctx.needs_input_grad
+        inner = n0 or n1 or nw or nb
         # relu without a residual: y > 0 is where its argument is, so y stands in for it
-        own = activation == "relu" and residual is None
-        y, z = hip.linear(x0, weight, bias, activation, residual, x1,
-                          want_z=inner and not own and hip.activation_code(activation) != 0)
-        ctx.activation = activation
-        ctx.bias = bias is not None
-        # x is read by the weight's gradient, the weight by x's
-        ctx.save_for_backward(x0 if inner else None, x1 if inner else None, weight if inner else None, y if own and inner else z)
+        own = act == 1 and residual is None
+        y, z = hip._linear(operands, act, bias, residual, inner and act != 0 and not own)
+        if inner:
+            x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev = operands
+            ctx.save_for_backward(x0, x1, w, y if own else z)
+            ctx.plan = (ld0, k0, ld1, k1, ldw, M, N, dt, dev, act)
         return y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy):
-        x0, x1, weight, z = ctx.saved_tensors
+        _once("linear")
         n0, n1, nw, nb, nr, _ = ctx.needs_input_grad
         dx0 = dx1 = dw = db = None
         if n0 or n1 or nw or nb:
-            dx0, dx1, dw, db = hip.linear_backward(gy, x0, weight, z, ctx.activation, x1, n0, n1, nw, nb)
+            x0, x1, w, z = ctx.saved_tensors
+            ld0, k0, ld1, k1, ldw, M, N, dt, dev, act = ctx.plan
+            dx0, dx1, dw, db = hip._linear_backward((x0, ld0, k0, x1, ld1, k1, w, ldw, M, N, dt, dev), act, gy, z, n0, n1, nw, nb)
         return dx0, dx1, dw, db, gy if nr else None, None
 
 
@@ -106,8 +113,8 @@ class _AddNormFn(torch.autograd.Function):
         return (y, h) if ctx.two else y
 
     @staticmethod
-    @once_differentiable
     def backward(ctx, gy, gh=None):
+        _once("add_rms_norm")
         nx, nw, nr, _ = ctx.needs_input_grad
         if gy is None:
             zero = None

@@ -223,6 +223,14 @@ def test_linear_gradients_against_differences(dev):
             assert abs(float((dt_.double() * d).sum()) - want) < 1e-4 * max(1.0, abs(want)), act
 
 
+def test_second_derivatives_are_refused(dev):
+    x = torch.randn(5, 8, device=dev, requires_grad=True)
+    w = torch.randn(8, 8, device=dev, requires_grad=True)
+    for y in (layers.linear(x, w, activation="silu"), layers.add_rms_norm(x, w[0])[0], layers.add_rms_norm(x, w[0], x)[0]):
+        with pytest.raises(NotImplementedError, match="first derivatives"):
+            torch.autograd.grad(y.sum(), x, create_graph=True)
+
+
 @pytest.mark.parametrize("dtype", list(TYPES))
 def test_linear_no_rows(dev, dtype):
     dt = TYPES[dtype]
