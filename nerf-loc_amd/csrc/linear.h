@@ -343,7 +343,7 @@ __device__ __forceinline__ i32x4 buffer_of(const void* p) {
     return r;
 }
 __device__ __forceinline__ void dma16(unsigned lds, unsigned voff, const i32x4& rsrc) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds), "v"(voff), "s"(rsrc) : "memory", "m0");
 }
 
 // The first `have` (1 .. CE - 1) elements at p, zeros behind them.  Not unrolled: it runs once at a row's end.
@@ -668,7 +668,8 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
 template <int DT, int ODT, int LAY, int BP, int BQ, int WVP, int WVQ, int WAY>
 int launch(GemmArgs& g, hipStream_t s) {
     const long long tp = (g.P + BP - 1) / BP, tq = (g.Q + BQ - 1) / BQ;
-    NERF_REQUIRE(tp * tq < (1ll << 31), "linear: %lld x %lld outputs are too many for one launch", g.P, g.Q);
+    // a launch counts its threads in 32 bits
+    NERF_REQUIRE(tp * tq < (1ll << 32) / (WVP * WVQ * 64), "linear: %lld x %lld outputs are too many for one launch", g.P, g.Q);
     g.tiles_p = (unsigned)tp;
     g.tiles_q = (unsigned)tq;
     auto k = gemm_kernel<DT, ODT, LAY, BP, BQ, WVP, WVQ, WAY>;

@@ -95,22 +95,23 @@ __global__ void __launch_bounds__(1024) part_sum_kernel(const float* parts, int 
         if (r == 0 && o < all) st_elem(out, (o / cols) * ldo + o % cols, s, DT);
     }
 }
-// The same for many elements and few parts: one thread each.
+// The same for many elements and few parts: one thread each, in turns (a launch counts its threads in 32 bits).
+constexpr long long WIDE_GROUPS = 1 << 20;
 template <int DT>
 __global__ void __launch_bounds__(256) part_sum_wide_kernel(const float* parts, int n, long long all, long long cols, void* out, long long ldo) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= all) return;
-    float s = 0.f;
+    for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < all; i += (long long)gridDim.x * 256) {
+        float s = 0.f;
 #pragma unroll 8
-    for (int k = 0; k < n; ++k) s += parts[(long long)k * all + i];
-    st_elem(out, (i / cols) * ldo + i % cols, s, DT);
+        for (int k = 0; k < n; ++k) s += parts[(long long)k * all + i];
+        st_elem(out, (i / cols) * ldo + i % cols, s, DT);
+    }
 }
 
 template <int DT>
 static void part_sum_launch(const float* parts, int n, long long all, long long cols, void* out, long long ldo, hipStream_t s) {
     // 64 threads an element pay where one each would leave the card half empty (128 parts of 65536: 16 us against 12)
     if (all <= 16384) hipLaunchKernelGGL(part_sum_kernel<DT>, dim3((unsigned)((all + 15) / 16)), dim3(1024), 0, s, parts, n, all, cols, out, ldo);
-    else hipLaunchKernelGGL(part_sum_wide_kernel<DT>, dim3((unsigned)((all + 255) / 256)), dim3(256), 0, s, parts, n, all, cols, out, ldo);
+    else hipLaunchKernelGGL(part_sum_wide_kernel<DT>, dim3((unsigned)std::min((all + 255) / 256, WIDE_GROUPS)), dim3(256), 0, s, parts, n, all, cols, out, ldo);
 }
 int part_sum(int dtype, const float* parts, int n, long long rows, long long cols, void* out, long long ldo, hipStream_t s) {
     switch (dtype) {
@@ -217,7 +218,7 @@ struct Product {
                 }
             }
         }
-        if (groups == 0 || groups >= (1ll << 31) || (layout == FWD && P <= FEW_ROWS)) return false;
+        if (groups == 0 || groups >= (1ll << 24) || (layout == FWD && P <= FEW_ROWS)) return false;
         copy_us += 5;
         const double aligned_us = products * 2 / (dtype == F32 ? 130e6 : 700e6);
         return copy_us < aligned_us * (dtype == F32 ? 0.4 : layout == FWD ? 1 : 4);

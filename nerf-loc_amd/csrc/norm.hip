@@ -128,7 +128,8 @@ __global__ void __launch_bounds__(ROWT < 256 ? 256 : ROWT) norm_kernel(const Nor
     constexpr int NT = ROWT < 256 ? 256 : ROWT;
     __shared__ float shared[16];
     const int t = threadIdx.x % ROWT;
-    const long long row = (long long)blockIdx.x * (NT / ROWT) + threadIdx.x / ROWT;
+    // two grid dimensions: a launch counts its threads in 32 bits along one
+    const long long row = ((long long)blockIdx.y * gridDim.x + blockIdx.x) * (NT / ROWT) + threadIdx.x / ROWT;
     const bool live = row < a.M;
     const long long rw = live ? row : a.M - 1;          // idle threads of the last workgroup follow its last row
     float h[VPT][8], ss = 0.f;
@@ -291,6 +292,7 @@ constexpr int NORM_MAX = 32768;      // 1024 threads x 4 x 8 columns
         else if ((N) <= 2048) { CALL(256, 1); }                    \
         else if ((N) <= 4096) { CALL(256, 2); }                    \
         else if ((N) <= 8192) { CALL(1024, 1); }                   \
+        else if ((N) <= 16384) { CALL(1024, 2); }                  \
         else { CALL(1024, 4); }                                    \
     } while (0)
 
@@ -306,7 +308,8 @@ static int norm_launch(const NormArgs& a, hipStream_t s) {
 #define NERF_CALL(T, V)                                                                                                   \
     {                                                                                                                     \
         constexpr int NT = T < 256 ? 256 : T;                                                                             \
-        const dim3 grid((unsigned)((a.M + NT / T - 1) / (NT / T)));                                                       \
+        const long long groups = (a.M + NT / T - 1) / (NT / T), wide = groups < (1ll << 20) ? groups : 1ll << 20;          \
+        const dim3 grid((unsigned)wide, (unsigned)((groups + wide - 1) / wide));                                          \
         if (a.q) hipLaunchKernelGGL((norm_kernel<DT, T, V, true>), grid, dim3(NT), 0, s, a);                              \
         else hipLaunchKernelGGL((norm_kernel<DT, T, V, false>), grid, dim3(NT), 0, s, a);                                 \
     }

@@ -339,6 +339,42 @@ def test_linear_offsets_beyond_32_bits(dev):
     assert torch.equal(hip.linear_backward(gy, x, w, want_x0=False, want_b=False)[2], hip.linear_backward(gy, c, w)[2])
 
 
+def test_linear_result_over_its_residual(dev):
+    """In the C interface y may be the residual itself: few rows, tiles, a cut product, and the streaming kernel."""
+    lib = hip.lib()
+    for m, n, k in ((5, 72, 64), (300, 200, 128), (73, 64, 4096), (131072, 256, 256), (65600, 64, 64)):
+        g = torch.Generator(device=dev).manual_seed(m)
+        x, w, r = (torch.randn(*s, device=dev, generator=g).bfloat16() for s in ((m, k), (n, k), (m, n)))
+        want, _ = hip.linear(x, w, None, "silu", r)
+        p = lambda t: t.data_ptr()
+        need = lib.nerf_linear_workspace_bytes(1, p(x), k, k, None, 0, 0, p(w), k, m, n)
+        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=dev)
+        assert lib.nerf_linear(1, p(x), k, k, None, 0, 0, p(w), k, None, 3, p(r), n, p(r), n, None, 0, m, n, p(ws), need,
+                               torch.cuda.current_stream().cuda_stream) == 0
+        assert torch.equal(r, want), (m, n, k)
+
+
+# the streaming kernels: every column and reduction group, partial last tiles, z kept or not
+@pytest.mark.parametrize("size", [(131072 + 77, 256, 256), (131072, 200, 136), (65536 + 31, 256, 64), (65536, 136, 128), (65536 + 1, 64, 256),
+                                  (65600, 8, 8), (65536, 104, 72), (70001, 128, 128)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_streaming_kernels(dev, dtype, size):
+    m, n, k = size
+    dt = TYPES[dtype]
+    for act, bias, residual in (("relu", True, False), ("gelu", False, True), ("silu", True, False), ("none", False, False)):
+        x, w, b, r, g = make(dev, dt, m, n, k, 0, bias, residual, 700 + n, grad=True)
+        y = layers.linear(x[0], w, b, act, r)
+        ref = Layer(x, w, b, r, act)
+        check(y.detach(), ref.y, ref.ey, ("y", act))
+        gy = torch.randn(m, n, device=dev, generator=g).to(dt)
+        dx, dw = torch.autograd.grad(y, [x[0], w], gy)
+        (rx, ex), (rw, ew), _ = ref.gradients(gy)
+        check(dx, rx, ex, ("dx", act))
+        check(dw, rw, ew, ("dw", act))
+        with torch.no_grad():
+            assert torch.equal(layers.linear(x[0], w, b, act, r), y)
+
+
 def test_linear_many_rows(dev):
     """More than 2^31 output elements: the last rows are where they belong."""
     m, n, k = (1 << 23) + 100, 264, 16
@@ -358,7 +394,7 @@ def norm64(x, w, r, eps):
 
 
 NORM_SIZES = [(1, 1), (1, 31), (5, 32), (300, 33), (64, 128), (67, 129), (3, 512), (130, 513), (9, 1024), (4099, 256), (6, 1025),
-              (11, 2048), (4, 2055), (1, 4096), (7, 4100), (3, 8192), (2, 9001), (2, 32768), (65, 7)]
+              (11, 2048), (4, 2055), (1, 4096), (7, 4100), (3, 8192), (2, 9001), (2, 16385), (2, 32768), (65, 7)]
 
 
 @pytest.mark.parametrize("size", NORM_SIZES, ids=lambda s: "x".join(map(str, s)))
@@ -394,6 +430,15 @@ def test_add_rms_norm_and_gradients(dev, dtype, size):
     check(got[1], dw, ew + u * (dw.abs() + ew) + t, "dw")
     if r is not None:
         assert torch.equal(got[0], got[2])
+
+
+def test_add_rms_norm_more_rows_than_one_grid_dimension(dev):
+    """More than 2^20 workgroups: the rows behind them are there."""
+    m = (1 << 26) + 1000
+    x = torch.full((m, 1), 3.0, dtype=torch.bfloat16, device=dev)
+    x[-1] = -2.0
+    y, _ = layers.add_rms_norm(x, torch.ones(1, dtype=torch.bfloat16, device=dev), eps=0.0)
+    assert float(y[:-1].min()) == float(y[:-1].max()) == 1.0 and float(y[-1]) == -1.0
 
 
 def test_add_rms_norm_of_zeros_and_non_finite_rows(dev):
