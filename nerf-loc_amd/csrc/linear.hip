@@ -200,10 +200,14 @@ struct Product {
     long long red[2];
     bool can_split;
 
-    // Unaligned rows cost a product about its own time over in the forward layout (each row's lines come twice; 0.4 times in
-    // float32), four times it where an operand lies reduction-major; a copy costs its bytes both ways and a launch.
-    // Measured: 4096 x 4096 x 4095 bf16 308 us as it lies, 151 us copied; 4097 x 515 x 1021 fp16 forward 23 and 31 us,
-    // dW 67 and 39 us.
+    // Unaligned rows are fetched line by line twice; a copy costs its bytes both ways and a launch.  Forward it pays once
+    // there are two tiles a compute unit (fewer wait for latency, not for bytes) and the copy is short against the product;
+    // where an operand lies reduction-major, and there is only one to copy, earlier.  Measured (us, as they lie and copied;
+    // copy over product by the estimates below):
+    //   forward fp16 4096 x 4096 x 4095 308 151   65536 x 256 x 319 66 56 (1.4)   4097 x 515 x 1021 23 29 (1.4, 297 tiles)
+    //   forward fp32 65536 x 256 x 319 160 141 (0.5)   30000 x 64 x 1001 48 82 (1.8)   2000 x 1000 x 1001 50 57 (0.3, 256 tiles)
+    //   dx fp16 4097 x 515 x 1021 43 29 (0.9)   1000 x 200 x 3001 16 18 (3.2)      dx fp32 8000 x 255 x 255 33 32 (0.6)
+    //   dW fp16 4097 x 515 x 1021 70 37 (1.4)   30000 x 64 x 1001 54 57 (5.3)      dW fp32 8000 x 255 x 255 43 41 (1.0)
     bool packs() const {
         const int e = elem_size(dtype);
         double copy_us = 0, products = 0;
@@ -220,8 +224,9 @@ struct Product {
         }
         if (groups == 0 || groups >= (1ll << 24) || (layout == FWD && P <= FEW_ROWS)) return false;
         copy_us += 5;
+        if (layout == FWD && ((P + 127) / 128) * ((Q + 63) / 64) < 512) return false;
         const double aligned_us = products * 2 / (dtype == F32 ? 130e6 : 700e6);
-        return copy_us < aligned_us * (dtype == F32 ? 0.4 : layout == FWD ? 1 : 4);
+        return copy_us < aligned_us * (dtype != F32 ? 2 : layout == DW ? 1.1 : 0.6);
     }
     int splits() const {
         if (!can_split || nseg != 1 || (layout == FWD && P <= FEW_ROWS)) return 1;

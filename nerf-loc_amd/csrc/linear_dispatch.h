@@ -33,7 +33,10 @@ template <int DT, int ODT, int LAY>
 int gemm_tiles(GemmArgs& g, hipStream_t s) {
     auto tiles = [&](int p, int q) { return ((g.P + p - 1) / p) * ((g.Q + q - 1) / q) * g.splits; };
     if (!dma_ok<DT>(LAY, g)) {
-        if (tiles(128, 128) >= 256) return launch<DT, ODT, LAY, 128, 128, 2, 2, REGS>(g, s);
+        // 128 columns a tile unless the last tile's empty part would be over a tenth of the work (130 columns: half of it)
+        const bool full = (g.Q + 127) / 128 * 128 * 10 <= (g.Q + 63) / 64 * 64 * 11;
+        if (full && tiles(128, 128) >= 256) return launch<DT, ODT, LAY, 128, 128, 2, 2, REGS>(g, s);
+        if (tiles(128, 64) >= 400) return launch<DT, ODT, LAY, 128, 64, 2, 2, REGS>(g, s);
         return launch<DT, ODT, LAY, 64, 64, 2, 2, REGS>(g, s);
     }
     if constexpr (LAY != DW && elem_size(DT) == 2) {

@@ -785,7 +785,8 @@ def _layer_input(x0, x1, weight):
 def linear(x0, weight, bias=None, activation=None, residual=None, x1=None, want_z=False):
     """act([x0 | x1] weight^T + bias) + residual on matrices [M, k0], [M, k1], [N, k0 + k1], [N], [M, N] of one type.
     Returns (y, z): z is the argument of act with want_z, else None."""
-    return _linear(_layer_input(x0, x1, weight), activation_code(activation), bias, residual, want_z)
+    act = activation_code(activation)
+    return _linear(_layer_input(x0, x1, weight), act, bias, residual, want_z)
 
 
 def _linear(operands, act, bias, residual, want_z):
@@ -806,7 +807,8 @@ def _linear(operands, act, bias, residual, want_z):
 def linear_backward(g, x0, weight, z=None, activation=None, x1=None, want_x0=True, want_x1=True, want_w=True, want_b=True):
     """Gradients of linear for g = dL/dy: (dx0, dx1, dweight, dbias), None where not wanted.  z: the argument of act that
     the forward gave (for relu without a residual, y)."""
-    return _linear_backward(_layer_input(x0, x1, weight), activation_code(activation), g, z, want_x0, want_x1, want_w, want_b)
+    act = activation_code(activation)
+    return _linear_backward(_layer_input(x0, x1, weight), act, g, z, want_x0, want_x1, want_w, want_b)
 
 
 def _linear_backward(operands, act, g, z, want_x0, want_x1, want_w, want_b):
