@@ -158,7 +158,6 @@ __device__ __forceinline__ float act_fn(float z, int act) {
 __device__ __forceinline__ float act_grad(float z, int act) {
     z = z > 100.f ? 100.f : z < -100.f ? -100.f : z;
     switch (act) {
-        case NERF_ACT_RELU: return z <= 0.f ? 0.f : 1.f;
         case NERF_ACT_GELU: {
             float e;
             const float c = normal_cdf(z, e);
@@ -170,6 +169,11 @@ __device__ __forceinline__ float act_grad(float z, int act) {
         }
         default: return 1.f;
     }
+}
+// g act'(z).  relu's 0 is chosen, not multiplied: an infinite g behind a closed relu stays out.
+__device__ __forceinline__ float through_act(float g, float z, int act) {
+    if (act == NERF_ACT_RELU) return z <= 0.f ? 0.f : g;
+    return g * act_grad(z, act);
 }
 // Eight columns of one row.  Both ways out (a whole group by 16-byte accesses, the last columns one by one) share the
 // arithmetic in between.

@@ -37,7 +37,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
                 if (a.act != NERF_ACT_NONE) {
                     ld8<DT>(a.z, p * a.ldz + q, z);
 #pragma unroll
-                    for (int j = 0; j < 8; ++j) g[j] *= act_grad(z[j], a.act);
+                    for (int j = 0; j < 8; ++j) g[j] = through_act(g[j], z[j], a.act);
                 }
                 if (a.gz) st8<DT>(a.gz, p * a.ldgz + q, g);
             } else {
@@ -46,7 +46,7 @@ __global__ void __launch_bounds__(256) act_grad_kernel(const ActGradArgs a) {
                     g[j] = 0.f;
                     if (q + j < a.N) {
                         g[j] = ld_elem(a.g, p * a.ldg + q + j, DT);
-                        if (a.act != NERF_ACT_NONE) g[j] *= act_grad(ld_elem(a.z, p * a.ldz + q + j, DT), a.act);
+                        if (a.act != NERF_ACT_NONE) g[j] = through_act(g[j], ld_elem(a.z, p * a.ldz + q + j, DT), a.act);
                     }
                     if (a.gz && q + j < a.ldgz) st_elem(a.gz, p * a.ldgz + q + j, g[j], DT);
                 }

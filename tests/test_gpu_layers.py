@@ -276,6 +276,27 @@ def test_linear_fp16_overflow_of_the_stored_argument(dev):
         assert gx.flatten().tolist() == [2.0, 0.0]
 
 
+@pytest.mark.parametrize("dtype", list(TYPES))
+def test_linear_relu_keeps_what_its_zero_meets_out(dev, dtype):
+    """An infinite or NaN gradient behind a closed ReLU reaches neither the inputs' nor the parameters' gradients: the
+    gradient is the one of a zero there, bit for bit, whether y or the stored argument says what is closed."""
+    dt = TYPES[dtype]
+    for m, n, k in ((9, 12, 24), (300, 72, 40)):
+        x, w, b, r, g = make(dev, dt, m, n, k, 0, True, True, 31)
+        gy = torch.randn(m, n, device=dev, generator=g).to(dt)
+        _, z = hip.linear(x[0], w, b, "relu", want_z=True)
+        shut = z <= 0
+        assert bool(shut.any()) and bool((~shut).any())
+        for fill in (float("inf"), float("-inf"), float("nan")):
+            for res in (None, r):
+                got, want = [], []
+                for out, fill_with in ((got, fill), (want, 0.0)):
+                    leaves = [t.clone().requires_grad_() for t in (x[0], w, b)]
+                    y = layers.linear(leaves[0], leaves[1], leaves[2], "relu", res)
+                    out += torch.autograd.grad(y, leaves, torch.where(shut, torch.tensor(fill_with, device=dev, dtype=dt), gy))
+                assert all(torch.equal(a, c) and bool(torch.isfinite(a).all()) for a, c in zip(got, want))
+
+
 def test_linear_same_result_every_time_and_under_graph_replay(dev):
     """No atomics: repeated calls agree bit for bit; a captured forward and backward replays to the eager result with eager
     work in between."""
