@@ -256,7 +256,8 @@ class NeRF(nn.Module):
             ev = torch.cuda.Event()
             ev.record(cur)
             flat = [t for v in out.values() for t in v]
-            self._pack_cache[("layers", prec)] = (key, out, cur, ev, flat)
+            # the parameters' memory stays alive with the entry, so that no other tensor can come to lie at its addresses
+            self._pack_cache[("layers", prec)] = (key, out, cur, ev, flat, [p.detach() for p in params])
         return out
 
     def _forward_layers(self, x, prec):

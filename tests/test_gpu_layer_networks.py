@@ -163,6 +163,60 @@ def test_cast_weights_follow_the_parameters(dev):
         assert torch.equal(c, d)
 
 
+def test_cast_weights_of_replaced_parameters(dev):
+    """A parameter whose memory is freed and replaced by a tensor that may come to lie at the same address, with the same
+    version: the cast weights are the new one's."""
+    net = build(dev, residual=True)
+    net.layer_precision = "bf16"
+    x = torch.rand(64, 90, device=dev)
+    with torch.no_grad():
+        for k in range(4):
+            net(x)
+            p = net.pts_linears[1].weight
+            shape, new = p.shape, np.random.RandomState(k).randn(*p.shape).astype(np.float32)
+            p.data = torch.empty(0, device=dev)
+            p.data = torch.from_numpy(new).to(dev)
+            got = net(x)
+            net.weights_changed()
+            assert p.shape == shape and torch.equal(got, net(x)), k
+
+
+def test_captured_training_step_of_a_network(dev):
+    """Forward, backward and the gradients' accumulation in a graph, with eager steps between the replays whose graphs
+    are gone when the capture begins."""
+    for residual in (False, True):
+        net = build(dev, residual=residual)
+        net.layer_precision = "bf16"
+        x, g = torch.rand(300, 90, device=dev), torch.randn(300, 4, device=dev)
+        params = list(net.parameters())
+
+        def step():
+            for p in params:
+                p.grad = None
+            net(x).backward(g)
+
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            step()
+        held = [p.grad for p in params]
+        for _ in range(3):
+            with torch.no_grad():
+                x.uniform_(-1, 1)
+                params[0].mul_(0.9)
+                for t in held:
+                    t.zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            got = [t.clone() for t in held]
+            step()
+            assert all(torch.equal(a, p.grad) for a, p in zip(got, params))
+
+
 def test_graph_capture_of_a_residual_network(dev):
     for prec in ("bf16", "q8"):
         net = build(dev, residual=True)
