@@ -9,8 +9,9 @@ renderer kernels do not cover it (other depths and widths, residual trunks), usa
 
 Tensors live on one GPU and share one type (float32, bfloat16, float16); sums, norms and scales are float32.  Leading
 dimensions are free.  The kernels run on the current stream of the tensors' device, allocate nothing but their results
-and scratch through torch, and can be captured in a graph.  Gradients are computed once (no second derivatives), and
-torch.autocast does not change the types here.
+and scratch through torch, and can be captured in a graph (a training step only once the results of eager steps on the
+same parameters are gone: torch accumulates a leaf's gradient on the stream of its first living graph).  Gradients are
+computed once (no second derivatives), and torch.autocast does not change the types here.
 """
 import torch
 
@@ -131,13 +132,13 @@ def add_rms_norm(x, weight, residual=None, eps=1e-6):
     without a residual h is x itself.  Differentiable in x, weight and residual; at most 32768 columns.
 
     In 16-bit types y comes from the float32 sum, h is that sum rounded, and the backward starts from the rounded h."""
+    _tensors(x=x, weight=weight, residual=residual)
     a = _flat(x, "x")
     r = None
     if residual is not None:
         if residual.shape != x.shape:
             raise ValueError("residual %s does not match x %s" % (tuple(residual.shape), tuple(x.shape)))
         r = _flat(residual, "residual")
-    _tensors(weight=weight)
     if _wants_grad(a, weight, r):
         out = _AddNormFn.apply(a, weight, r, float(eps))
         y, h = out if r is not None else (out, x)
@@ -188,6 +189,9 @@ def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=Non
 @torch.no_grad()
 def quantize_weight(weight):
     """(wq float8_e4m3fn [N, K], w_scale float32 [N]) for linear_q8, made once per weight version with torch."""
+    _tensors(weight=weight)
+    if weight.dim() != 2 or weight.shape[1] < 1:
+        raise ValueError("weight must be a matrix with columns, got %s" % (tuple(weight.shape),))
     w = weight.float()
     scale = (w.abs().amax(-1) / 448.0).clamp_min(2.0 ** -126)
     return (w / scale[:, None]).to(torch.float8_e4m3fn), scale

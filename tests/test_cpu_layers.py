@@ -121,6 +121,21 @@ def test_python_entries_refuse():
         layers.add_rms_norm_q8(x.requires_grad_(), torch.ones(8))
 
 
+def test_python_entries_name_the_operand_that_is_no_tensor():
+    x, w, f8 = torch.zeros(3, 8), torch.ones(8), torch.float8_e4m3fn
+    for call, name in ((lambda: layers.add_rms_norm(3, w), "x"), (lambda: layers.add_rms_norm(x, 3), "weight"),
+                       (lambda: layers.add_rms_norm(x, w, 3), "residual"), (lambda: layers.add_rms_norm_q8(x, w, [1]), "residual"),
+                       (lambda: layers.linear(x, x, bias=3), "bias"), (lambda: layers.linear(x, x, residual=3), "residual"),
+                       (lambda: layers.linear((x, 3), x), "the second piece of x"),
+                       (lambda: layers.linear_q8(x.to(f8), 3, x.to(f8), torch.ones(3)), "x_scale"),
+                       (lambda: layers.quantize_weight(3), "weight")):
+        with pytest.raises(TypeError, match="%s must be a torch.Tensor" % name):
+            call()
+    for bad in (torch.zeros(8), torch.zeros(2, 3, 4), torch.zeros(4, 0)):
+        with pytest.raises(ValueError, match="weight must be a matrix"):
+            layers.quantize_weight(bad)
+
+
 def test_quantize_weight_on_the_cpu():
     """Setup work in torch: runs anywhere.  Rows of zeros divide by the smallest scale."""
     w = torch.tensor([[0.0, 0.0], [448.0, 1.0], [-7.0, 3.5]])
