@@ -328,7 +328,9 @@ int nerf_linear_backward(int dtype, const void* g, long long ldg, const void* z,
                          void* dw, void* db, long long M, int N, void* workspace, size_t workspace_bytes, void* stream);
 
 /* nerf_linear on 8-bit operands (e4m3: four exponent bits, no infinities, largest 448): xq [M,K] and wq [N,K] hold
- * numbers that stand for x_scale[m] xq and w_scale[n] wq.  y, bias and residual are of type out_dtype.               */
+ * numbers that stand for x_scale[m] xq and w_scale[n] wq.  y, bias and residual are of type out_dtype.  Above 64 rows a
+ * 16-bit result's products are added in eights at 2^-13 of the eight's largest (the matrix instruction's way), the eights
+ * in float32; for a float32 result, and few rows, every product is added in float32.                                 */
 size_t nerf_linear_q8_workspace_bytes(const void* xq, long long ldx, const void* wq, long long ldw, long long M, int N, int K);
 int nerf_linear_q8(const void* xq, long long ldx, const float* x_scale, const void* wq, long long ldw,
                    const float* w_scale, int out_dtype, const void* bias, int activation, const void* residual,

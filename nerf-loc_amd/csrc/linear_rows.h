@@ -79,10 +79,10 @@ __device__ __forceinline__ void from_row(const u32x4& v, unsigned (&lo)[2], unsi
     swap32(hi[0], hi[1]);
 }
 
-// H x NF 16-column fragments of C, KS 32-element steps of the reduction; TB: B lies reduction-major.  With H = 2 two waves
-// share the rows and halve the columns: 32 rows x 256 columns of sums, 256 inputs of 32 rows and the weights' fragments
-// do not fit one wave's 256 registers (measured with spills: 310 us for 786432 x 256 x 256).  Z, RES: the epilogue stores
-// its argument, adds a residual.
+// H x NF 16-column fragments of C, KS 32-element steps of the reduction; TB: B lies reduction-major.  With H = 2 (129 to
+// 256 outputs with a residual; without one panel_kernel takes them) two waves share the rows and halve the columns: 32 rows
+// x 256 columns of sums, 256 inputs of 32 rows and the weights' fragments do not fit one wave's 256 registers (measured
+// with spills: 310 us for 786432 x 256 x 256, against 212).  Z, RES: the epilogue stores its argument, adds a residual.
 //
 // From a block's first load to its last store there is no branch: loads and stores retire in order, and behind a branch
 // that may or may not have issued some the compiler waits as if it had issued none, that is, for the stores of the block

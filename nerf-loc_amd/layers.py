@@ -172,7 +172,10 @@ def add_rms_norm_q8(x, weight, residual=None, eps=1e-6):
 
 def linear_q8(xq, x_scale, wq, w_scale, bias=None, activation=None, residual=None, out_dtype=torch.bfloat16):
     """act(x W^T + bias) + residual with x = x_scale xq (xq float8_e4m3fn [..., K], x_scale float32 [...]) and
-    W = w_scale wq ([N, K], [N]); bias, residual and the result are of out_dtype.  No gradient."""
+    W = w_scale wq ([N, K], [N]); bias, residual and the result are of out_dtype.  No gradient.
+
+    Above 64 rows a 16-bit result's products are added by the 8-bit matrix instruction, eight at a time at 2^-13 of the
+    eight's largest, the eights in float32; a float32 result, and few rows, add every product in float32."""
     _tensors(xq=xq, x_scale=x_scale, wq=wq, w_scale=w_scale, bias=bias, residual=residual)
     _no_grad("linear_q8", x_scale, w_scale, bias, residual)
     a = _flat(xq, "xq")
