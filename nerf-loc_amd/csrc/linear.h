@@ -72,6 +72,16 @@ int gemm_f32(int layout, GemmArgs& g, hipStream_t s);
 int gemm_bf16(int layout, GemmArgs& g, hipStream_t s);
 int gemm_f16(int layout, GemmArgs& g, hipStream_t s);
 int gemm_f8(GemmArgs& g, hipStream_t s);                 // out_dt names the epilogue's type
+// dx = (g act'(z)) W in one kernel with what else the backward needs of gz = g act'(z) (linear_rows.h)
+struct PanelGrad {
+    const void* z;
+    void* gz;                    // [P][ldgz], written
+    long long ldz, ldgz;
+    float* colsum;               // [PANEL_GRAD_GROUPS][red], written, or null
+};
+constexpr int PANEL_GRAD_GROUPS = 256;
+int panel_grad_bf16(GemmArgs& g, const PanelGrad& a, hipStream_t s);
+int panel_grad_f16(GemmArgs& g, const PanelGrad& a, hipStream_t s);
 // out [rows, cols] (rows ldo apart) = sum over n parts [rows][cols], in a fixed order (linear.hip)
 int part_sum(int dtype, const float* parts, int n, long long rows, long long cols, void* out, long long ldo, hipStream_t s);
 

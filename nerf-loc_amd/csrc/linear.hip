@@ -385,6 +385,18 @@ struct Backward {
     }
 };
 
+// Whether panel_grad_kernel takes the gradient with respect to an input piece: from 32768 rows on, and 256 outputs and
+// inputs together.  Measured (us, the whole backward apart and with it; relu, gelu in bf16):
+//   16384 x 256 x 256    36  36    37  38      196608 x 256 x 256   174 144   179 152     196608 x 256 x 64   128  99   134 116
+//   32768 x 256 x 256    53  49    55  54      786432 x 256 x 256   647 513   662 516     196608 x 128 x 128   89  84    98  91
+//   65536 x 256 x 256    87  77    89  83       65536 x 256 x 128    64  58    67  66      65536 x 128 x 64    34  35    37  39
+static bool panel_grad_ok(const GemmArgs& g, const PanelGrad& a) {
+    const Seg& s = g.seg[0];
+    auto rows = [](const void* p, long long ld) { return ((uintptr_t)p & 15) == 0 && ld % 8 == 0 && ld < (1ll << 22); };
+    return g.act != NERF_ACT_NONE && g.P >= 32768 && s.red > 64 && s.red <= 256 && s.red % 8 == 0 && g.Q <= 256 && g.Q % 8 == 0 && s.red + g.Q >= 256 &&
+           rows(s.a, s.lda) && rows(s.b, s.ldb) && rows(g.y, g.ldy) && rows(a.z, a.ldz) && rows(a.gz, a.ldgz);
+}
+
 static bool dtype_ok(int d) { return d == F32 || d == BF16 || d == F16; }
 static bool act_ok(int a) { return a >= NERF_ACT_NONE && a <= NERF_ACT_SILU; }
 
@@ -513,7 +525,28 @@ extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, con
 
     const bool through = bw.through() && (dx0 || dx1 || dw);
     float* colsum = reinterpret_cast<float*>(base + bw.colsum_at());
-    if (through || db) {
+    int fused = -1;              // the piece whose dx comes with gz
+    for (int piece = 0; piece < 2 && through && e == 2 && fused < 0; ++piece) {
+        void* dx = piece ? dx1 : dx0;
+        if (!dx) continue;
+        const Product f = bw.dx(piece, base);
+        GemmArgs a = {};
+        a.seg[0] = {g, f.b[0].p, ldg, ldw, N, false, false};
+        a.nseg = 1;
+        a.P = M;
+        a.Q = f.Q;
+        a.splits = 1;
+        a.y = dx;
+        a.ldy = piece ? lddx1 : lddx0;
+        a.act = activation;
+        const PanelGrad pg = {z, base, ldz, bw.ldgz(), db ? colsum : nullptr};
+        if (!panel_grad_ok(a, pg)) continue;
+        fused = piece;
+        int rc = dtype == BF16 ? panel_grad_bf16(a, pg, s) : panel_grad_f16(a, pg, s);
+        if (rc == NERF_OK && db) rc = part_sum(dtype, colsum, PANEL_GRAD_GROUPS, 1, N, db, N, s);
+        if (rc != NERF_OK) return rc;
+    }
+    if (fused < 0 && (through || db)) {
         ActGradArgs a = {};
         a.g = g;
         a.z = z;
@@ -544,7 +577,8 @@ extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, con
     for (int piece = 0; piece < 2; ++piece) {
         const int k = piece ? k1 : k0;
         if (k == 0) continue;
-        if (void* dx = piece ? dx1 : dx0) {
+        void* dx = piece ? dx1 : dx0;
+        if (dx && piece != fused) {
             GemmArgs a = {};
             a.y = dx;
             a.ldy = piece ? lddx1 : lddx0;

@@ -662,3 +662,30 @@ def test_linear_q8_cut_and_copied(dev):
         check(layers.linear_q8(xq, xs, wq, ws, out_dtype=torch.float32), z, ez + E * z.abs(), "float32")
         ez = ez + group_cut(X, W) * xs.double()[:, None] * ws.double()
         check(layers.linear_q8(xq, xs, wq, ws), z, ez + half_step(torch.bfloat16) * (z.abs() + ez), "bf16")
+
+
+# the input gradient formed together with the pass through the activation: both widths of its reduction, partial last tiles,
+# the first, the second or both pieces wide enough for it, columns that end inside a group of the weights
+@pytest.mark.parametrize("size", [(131072 + 45, 256, 256, 0), (131072, 72, 184, 0), (131072 + 1, 128, 200, 0), (140000, 136, 256, 0),
+                                  (131103, 256, 63, 256), (131072, 200, 256, 136), (32768, 256, 8, 0), (32768 + 31, 248, 72, 0),
+                                  (40001, 128, 128, 0)], ids=lambda s: "x".join(map(str, s)))
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_gradient_through_the_activation_and_the_input_at_once(dev, dtype, size):
+    m, n, k, k2 = size
+    dt = TYPES[dtype]
+    for act, residual in (("relu", False), ("relu", True), ("gelu", False), ("silu", False)):
+        x, w, b, r, g = make(dev, dt, m, n, k, k2, True, residual, 900 + n, grad=True)
+        y = layers.linear(x[0] if k2 == 0 else tuple(x), w, b, act, r)
+        gy = torch.randn(m, n, device=dev, generator=g).to(dt)
+        got = torch.autograd.grad(y, x + [w, b], gy, retain_graph=True)
+        (dx, ex), (dw, ew), (db, eb) = Layer(x, w, b, r, act).gradients(gy)
+        check(torch.cat(got[:len(x)], -1), dx, ex, ("dx", act))
+        check(got[-2], dw, ew, ("dw", act))
+        check(got[-1], db, eb, ("db", act))
+        again = torch.autograd.grad(y, x + [w, b], gy, retain_graph=True)
+        assert all(torch.equal(a, c) for a, c in zip(got, again))
+        # without the parameters' gradients, and from a gradient that lies in wider rows
+        wide = torch.full((m, n + 24), float("nan"), device=dev, dtype=dt)
+        wide[:, 8:8 + n] = gy
+        alone = torch.autograd.grad(y, x[-1], wide[:, 8:8 + n])[0]
+        assert torch.equal(alone, got[len(x) - 1])

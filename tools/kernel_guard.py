@@ -31,7 +31,7 @@ LLVM = "/opt/rocm/lib/llvm/bin"
 # kernels with hand-counted waits (substrings of the demangled-ish symbol)
 GUARDED = ("wgrad_kernel", "wgrad16_kernel", "mlp16_bf16_kernel", "mlp_split_kernel", "mlp_split_train_kernel", "mlp_split_dgrad_kernel",
            "mlp_bf16_kernel",
-           "mlp_dgrad_bf16_kernel", "panel_kernel")
+           "mlp_dgrad_bf16_kernel", "panel_kernel", "panel_grad_kernel")
 # of these, the kernels whose EVERY load into registers is hand-counted inline asm: only there is the linear walk of the
 # instruction stream meaningful (compiler-managed loads sit in branches a linear walk cannot follow, and the compiler
 # places their waits itself); the LDS-DMA of the other kernels has no destination register to watch
