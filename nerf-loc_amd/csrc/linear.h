@@ -63,6 +63,10 @@ inline int splits_for(long long P, long long Q, long long red, int elem) {
     const long long s = 256 / tiles < k_tiles / 4 ? 256 / tiles : k_tiles / 4;
     return s < 1 ? 1 : (int)s;
 }
+// Whether tiles of bp x bq cover [P, Q] with at most an eighth more than those of 128 x 64 would
+inline bool tile_fits(long long P, long long Q, int bp, int bq) {
+    return (P + bp - 1) / bp * bp * ((Q + bq - 1) / bq * bq) * 8 <= (P + 127) / 128 * 128 * ((Q + 63) / 64 * 64) * 9;
+}
 constexpr long long FEW_ROWS = 64;       // up to here few_rows_kernel takes the forward product
 
 // what the three products need of the operands' layouts
@@ -518,19 +522,22 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int wp = (wave / WVQ) * WP, wq = (wave % WVQ) * WQ;
 
-    // workgroup -> tile: consecutive workgroups go to the 8 XCDs in turn, so XCD x takes the x-th eighth of the tiles,
-    // and within it walks 8 rows of tiles column by column: its L2 then holds both operands' panels
-    const unsigned n_tiles = g.tiles_p * g.tiles_q;
-    unsigned t = blockIdx.x;
+    // workgroup -> part and tile: consecutive workgroups go to the 8 XCDs in turn, so XCD x takes the x-th eighth of them,
+    // part by part, and within one walks 8 rows of tiles column by column: its L2 then holds both operands' panels (dW of
+    // 196608 x 256 x 256 bf16 53 us, with the tiles of a part on XCDs of their own 61)
+    const unsigned n_tiles = g.tiles_p * g.tiles_q, all = n_tiles * gridDim.y;
+    unsigned t = blockIdx.y * n_tiles + blockIdx.x;
     {
-        const unsigned x = t & 7, i = t >> 3, each = n_tiles >> 3, more = n_tiles & 7;
+        const unsigned x = t & 7, i = t >> 3, each = all >> 3, more = all & 7;
         t = x * each + (x < more ? x : more) + i;
     }
+    const unsigned part = gridDim.y > 1 ? t / n_tiles : 0;
+    t -= part * n_tiles;
     const unsigned per = 8 * g.tiles_q, grp = t / per, first = grp * 8;
     const unsigned rows = g.tiles_p - first < 8 ? g.tiles_p - first : 8, in = t - grp * per;
     const long long p0 = (long long)(first + in % rows) * BP, q0 = (long long)(in / rows) * BQ;
 
-    const long long r_lo = g.splits > 1 ? (long long)blockIdx.y * g.red_part : 0;
+    const long long r_lo = (long long)part * g.red_part;
     long long red[2] = {g.seg[0].red, g.nseg > 1 ? g.seg[1].red : 0};
     if (g.splits > 1) red[0] = red[0] - r_lo < g.red_part ? red[0] - r_lo : g.red_part;
     const int nt0 = (int)((red[0] + BK - 1) / BK), nt = nt0 + (int)((red[1] + BK - 1) / BK);
@@ -683,7 +690,7 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
             for (int j = 0; j < 4; ++j) { v[j] = lo[j]; v[4 + j] = hi[j]; }
             if (p < g.P && q < g.Q) {
                 if (g.partial) {
-                    float* o = g.partial + ((long long)blockIdx.y * g.P + p) * g.Q + q;
+                    float* o = g.partial + ((long long)part * g.P + p) * g.Q + q;
                     if (q + 8 <= g.Q) __builtin_memcpy(o, v, 32);
                     else {
 #pragma unroll

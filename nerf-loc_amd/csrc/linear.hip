@@ -270,7 +270,7 @@ struct Product {
         g.Q = Q;
         g.splits = given;
         if (sp == 1) return dispatch_gemm(dtype, layout, g, st);
-        const long long unit = 128;              // a multiple of every type's k-tile
+        const long long unit = 128;              // whole k-tiles; shorter parts cost more to add up than they save
         g.red_part = ((red[0] + sp - 1) / sp + unit - 1) / unit * unit;
         g.splits = (int)((red[0] + g.red_part - 1) / g.red_part);
         g.partial = reinterpret_cast<float*>(ws);
@@ -317,11 +317,13 @@ static long long colsum_rows(long long M) {
 }
 static int colsum_blocks(long long M) { return M ? (int)((M + colsum_rows(M) - 1) / colsum_rows(M)) : 0; }
 
-// dW = gz^T x has a long reduction (the samples) and few outputs: cut until about 512 workgroups of 128 x 128 have work,
-// not below 512 samples a part.
+// dW = gz^T x has a long reduction (the samples) and few outputs: cut into as many parts as fill the card once (one tile
+// of 256 x 128 a compute unit, three of 128 x 64), not below 512 samples a part.  (One part too many is a second round:
+// 65536 x 256 x 320 float32 in 258 workgroups of 256 x 128 217 us, in 255 117.)
 static int dw_splits(long long M, long long N, long long K) {
-    const long long tiles = ((N + 127) / 128) * ((K + 127) / 128);
-    long long s = (512 + tiles - 1) / tiles;
+    const bool wide = tile_fits(N, K, 256, 128);
+    const long long tiles = wide ? ((N + 255) / 256) * ((K + 127) / 128) : ((N + 127) / 128) * ((K + 63) / 64);
+    long long s = (wide ? 256 : 768) / tiles;
     const long long most = (M + 511) / 512;
     if (s > most) s = most;
     return s < 1 ? 1 : (int)s;
@@ -591,7 +593,7 @@ extern "C" int nerf_linear_backward(int dtype, const void* g, long long ldg, con
             char* out = static_cast<char*>(dw) + (piece ? (size_t)k0 * e : 0);
             int sp = dw_splits(M, N, k);
             if (sp > 1) {
-                const long long unit = 128;              // a multiple of every type's k-tile
+                const long long unit = 128 / e;          // whole k-tiles
                 a.red_part = ((M + sp - 1) / sp + unit - 1) / unit * unit;
                 sp = (int)((M + a.red_part - 1) / a.red_part);
                 a.partial = reinterpret_cast<float*>(base + bw.scratch_at() + f.bytes());

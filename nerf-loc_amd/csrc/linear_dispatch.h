@@ -25,6 +25,9 @@ inline bool dma_ok(int layout, const GemmArgs& g) {
 // The tile.  256 x 256 reads its operands least often and pays once every compute unit has one and sixteen k-tiles to work
 // through; 256 x 128 the same with half the outputs; below, and for short reductions, where filling and draining the
 // pipeline is the time, 128 x 64 runs three workgroups a unit beside each other, and 64 x 64 spreads what little there is.
+// Tiles that would cover over an eighth more than the outputs need are left to the smaller ones, but for 256 x 256 in 16 and
+// 8 bits, where reading less outweighs it (32768 x 576 x 4096 bf16 204 us, with 256 x 128 228; 65536 x 320 x 2048 float32 994
+// and with 128 x 64 699; its dW 65536 x 128 x 320 151 and 68).
 // Measured (us; 256 x 256, 256 x 128, 128 x 128, 128 x 64, 64 x 64):
 //   bf16 8192 x 4096 x 4096    258  295  318    -  444      bf16 4096 x 2048 x 2048   61  42  48  53  61
 //   bf16 4096 x 1024 x 4096    110   70   61   53   62      fp32 65536 x 256 x 320   111 107 108  98 101
@@ -45,9 +48,13 @@ int gemm_tiles(GemmArgs& g, hipStream_t s) {
     const long long red = g.splits > 1 ? g.red_part : g.seg[0].red + (g.nseg > 1 ? g.seg[1].red : 0);
     const bool deep = red * elem_size(DT) >= 16 * 128;
     if constexpr (LAY == FWD && DT != F8W) {       // the reduction-major layouts and the widened operands do not fit its registers
-        if (deep && tiles(256, 256) >= 256) return launch<DT, ODT, LAY, 256, 256, 2, 4, DMA16>(g, s);
+        // float32 is bound by its matrix instructions: whole rounds of the card count (16384 x 1096 x 1024 511 us, with
+        // 256 x 128 407), and columns in vain (65536 x 192 x 1024 264, with 128 x 64 207)
+        const bool worth = DT != F32 || (tile_fits(g.P, g.Q, 256, 256) && (tiles(256, 256) + 255) / 256 * 2 <= (tiles(256, 128) + 255) / 256);
+        if (deep && worth && tiles(256, 256) >= 256) return launch<DT, ODT, LAY, 256, 256, 2, 4, DMA16>(g, s);
     }
-    if (deep && tiles(256, 128) >= 256) return launch<DT, ODT, LAY, 256, 128, 4, 2, DMA16>(g, s);
+    // dW is cut to fill the card once, its last parts may be empty
+    if (deep && tile_fits(g.P, g.Q, 256, 128) && tiles(256, 128) >= (LAY == DW ? 192 : 256)) return launch<DT, ODT, LAY, 256, 128, 4, 2, DMA16>(g, s);
     if (tiles(128, 64) >= 400) return launch<DT, ODT, LAY, 128, 64, 2, 2, DMA16>(g, s);
     return launch<DT, ODT, LAY, 64, 64, 2, 2, DMA16>(g, s);
 }
