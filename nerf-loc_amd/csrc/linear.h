@@ -514,8 +514,9 @@ __global__ void __launch_bounds__(WVP* WVQ * 64) gemm_kernel(const GemmArgs g) {
     constexpr int BK = TAt::BK, E = TAt::E;
     constexpr int STAGE = TAt::BYTES + TBt::BYTES;
     // three k-tiles in LDS for the smallest tile, whose k-tiles are worked off faster than memory answers (512 x 512 x 4096
-    // bf16 18.9 -> 15.7 us, gradients of 1000 x 1000 x 1000 fp16 30.1 -> 27.6); larger tiles gain nothing from it
-    constexpr int NS = WAY != REGS && !is_f8(DT) && BP == 64 && BQ == 64 ? 3 : 2;
+    // bf16 18.9 -> 15.7 us, gradients of 1000 x 1000 x 1000 fp16 30.1 -> 27.6), and for dW's largest, whose operands come from memory once (786432 x
+    // 256 x 256 bf16 183 -> 159, 65536 x 1024 x 1024 178 -> 157; float32 223 -> 225); the others gain nothing from it
+    constexpr int NS = WAY != REGS && !is_f8(DT) && ((BP == 64 && BQ == 64) || (LAY == DW && BP == 256 && E == 2)) ? 3 : 2;
     constexpr int EPI = WVP * WVQ * epi_bytes<WP, WQ>(), LDS = NS * STAGE > EPI ? NS * STAGE : EPI;
     static_assert(LDS <= 160 * 1024, "LDS of one compute unit");
     __shared__ __align__(1024) unsigned char smem[LDS];
