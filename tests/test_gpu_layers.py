@@ -689,3 +689,45 @@ def test_linear_gradient_through_the_activation_and_the_input_at_once(dev, dtype
         wide[:, 8:8 + n] = gy
         alone = torch.autograd.grad(y, x[-1], wide[:, 8:8 + n])[0]
         assert torch.equal(alone, got[len(x) - 1])
+
+
+@pytest.mark.parametrize("dtype", ["bf16", "fp16"])
+def test_linear_relu_keeps_out_what_its_zero_meets_with_many_rows(dev, dtype):
+    """The same on the streaming kernel: infinities and NaN behind closed ReLUs leave every gradient as zeros there do."""
+    dt = TYPES[dtype]
+    m, n, k = 32768 + 5, 136, 128
+    x, w, b, _, g = make(dev, dt, m, n, k, 0, True, False, 32)
+    gy = torch.randn(m, n, device=dev, generator=g).to(dt)
+    y, _ = hip.linear(x[0], w, b, "relu")
+    for fill in (float("inf"), float("nan")):
+        got, want = (hip.linear_backward(torch.where(y <= 0, torch.tensor(v, device=dev, dtype=dt), gy), x[0], w, y, "relu") for v in (fill, 0.0))
+        for i in (0, 2, 3):
+            assert torch.equal(got[i], want[i]) and bool(torch.isfinite(got[i]).all()), (fill, i)
+
+
+def test_linear_training_streams_in_two_graphs_at_once(dev):
+    """Two captured backward passes of the streaming kernels, replayed on two streams at a time: each has its own scratch."""
+    cases = []
+    for seed in (41, 42):
+        x, w, b, _, g = make(dev, torch.bfloat16, 40000, 256, 256, 0, True, False, seed)
+        gy = torch.randn(40000, 256, device=dev, generator=g).bfloat16()
+        y, z = hip.linear(x[0], w, b, "gelu", want_z=True)
+        call = lambda x=x, w=w, z=z, gy=gy: [t for t in hip.linear_backward(gy, x[0], w, z, "gelu") if t is not None]
+        want = call()
+        graph, side = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+        torch.cuda.synchronize()
+        with torch.cuda.graph(graph):
+            held = call()
+        cases.append((graph, side, held, want, gy, call))
+    for k in range(3):
+        for graph, side, held, want, gy, call in cases:
+            for t in held:
+                t.zero_()
+        torch.cuda.synchronize()
+        for graph, side, held, want, gy, call in cases:
+            with torch.cuda.stream(side):
+                graph.replay()
+        torch.cuda.synchronize()
+        for graph, side, held, want, gy, call in cases:
+            assert all(torch.equal(a, c) for a, c in zip(held, want)), k
+            assert all(torch.equal(a, c) for a, c in zip(call(), want)), k
